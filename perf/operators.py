@@ -1,6 +1,6 @@
 """Cases of the serving operators: the 4-bit KV cache (append, read back, attention over it) and token sampling.
 
-Formats and formulas, as include/bf16x_serve.h has them:
+Formats and formulas, as include/bf16x_llama.h has them:
 
   cache    codes uint8 [batch, kv_heads, max_len, D / 2], scales fp16 [batch, kv_heads, max_len, D / 32, 2] = (scale,
            minimum) of each group of 32 values of a row; value = minimum + scale * code.  The 8 codes of values 8w ..
