@@ -108,6 +108,16 @@ PROTOTYPES = {
                                                 _P, _P, _P, _c_i64, _P, _P, _P, _c_i64, _P]),
     "bf16x_greedy_workspace_bytes": (_c_i64, []),
     "bf16x_greedy": (ctypes.c_int, [_P, _c_i64, _P, _P, _P, _c_i64, _P, _c_i64, _P]),
+    # include/bf16x_llama.h, serving
+    "bf16x_kv4_append": (ctypes.c_int, [_P, _c_i64, _c_i64, _c_i64] * 3 + [_c_i32] + [_c_i64] * 6 + [_P, _P, _c_i64] +
+                         [_P] * 6),
+    "bf16x_kv4_read": (ctypes.c_int, [_P] * 4 + [_c_i64] * 5 + [_P, _c_i32, _P, _P, _P]),
+    "bf16x_kv4_attention_workspace": (_c_i64, [_c_i64] * 6),
+    "bf16x_kv4_attention": (ctypes.c_int, [_P, _c_i64, _c_i64, _c_i64, _c_i32] + [_c_i64] * 6 + [_P] * 6 +
+                            [_c_i64, ctypes.c_float, _P, _P, _c_i64, _P]),
+    "bf16x_sample_workspace": (_c_i64, [_c_i64, _c_i64]),
+    "bf16x_sample": (ctypes.c_int, [_P, _c_i32, _c_i64, _c_i64, _c_i64, _P, _c_i64, _P, _P, _P, _P, _P, _c_i64, _P,
+                                    _c_i64, _P]),
     # kernel-choice overrides (include/bf16x_hip.h)
     "bf16x_set_tuning": (ctypes.c_int, [_c_i32, _c_i64]),
     "bf16x_get_tuning": (_c_i64, [_c_i32]),

@@ -4,9 +4,9 @@
 
 Every HIP source is compiled for gfx950 with packed-fp32 instruction
 selection disabled, host C++ sources with the same driver, and the objects
-are linked into bfloat16x_amd/libbf16x_hip.so.  csrc/host_ext.cpp, the CPython
-module over torch's C++ API, is compiled with g++ into bfloat16x_amd/_host.so.  Objects go to _build/
-(ignored by git).
+are linked into bfloat16x_amd/libbf16x_hip.so.  csrc/host_ext.cpp and
+csrc/host_serve.cpp, the CPython module over torch's C++ API, are compiled with g++ into
+bfloat16x_amd/_host.so.  Objects go to _build/ (ignored by git).
 """
 from __future__ import annotations
 
@@ -22,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libbf16x_hip.so")
-HOST_SRC = os.path.join(CSRC, "host_ext.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host_ext.cpp", "host_serve.cpp")]
 HOST_OUT = os.path.join(HERE, "_host.so")
 BUILD_DIR = os.path.join(ROOT, "_build", "bf16x_hip")
 ARCH = "gfx950"
@@ -66,24 +66,32 @@ def _build_host(verbose: bool) -> None:
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = HOST_OUT + ".tmp"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
-           "-I" + os.path.join(ROOT, "include"), "-isystem", inc, "-isystem",
-           os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
-           "-isystem", "/opt/rocm/include", HOST_SRC, "-o", tmp, "-L" + tlib, "-ltorch_python", "-ltorch_cpu",
-           "-ltorch", "-lc10", "-lc10_hip", "-L" + HERE, "-lbf16x_hip", "-Wl,-rpath,$ORIGIN"]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("g++ failed on host_ext.cpp:\n" + r.stdout + r.stderr)
+    cxx = os.environ.get("CXX", "g++")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
+             "-I" + os.path.join(ROOT, "include"), "-isystem", inc, "-isystem",
+             os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
+             "-isystem", "/opt/rocm/include"]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("g++ failed on the host module:\n" + r.stdout + r.stderr)
+
+    objs = [os.path.join(BUILD_DIR, os.path.basename(src) + ".o") for src in HOST_SRCS]
+    with cf.ThreadPoolExecutor(max_workers=len(objs)) as ex:
+        list(ex.map(lambda so: run([cxx] + flags + ["-c", so[0], "-o", so[1]]), zip(HOST_SRCS, objs)))
+    run([cxx, "-shared"] + objs + ["-o", tmp, "-L" + tlib, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10",
+                                   "-lc10_hip", "-L" + HERE, "-lbf16x_hip", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, HOST_OUT)
 
 
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD_DIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
-    srcs.remove(HOST_SRC)
+    srcs = [s for s in srcs if s not in HOST_SRCS]
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
     tmp = OUT + ".tmp"

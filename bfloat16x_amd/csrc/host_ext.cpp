@@ -6,24 +6,21 @@
 //   gemv(...)       the checks, the output and the launch of ops.bf16x_gemv,
 //   plain(...)      the checks of the other wrappers (device, type, layout),
 //   stream(device)  torch's current stream,
-//   and the hot C-ABI entries with tensors accepted for their pointers.
+//   and the hot C-ABI entries with tensors accepted for their pointers;
+//   host_serve.cpp adds the serving operators.
 // gemv and plain only say yes to ordinary tensors that the entry takes as they
 // are; on anything else (another type or layout, a wrapped or fake tensor, an
 // error) they answer None / False and the wrapper's Python path runs, with its
 // conversions and its exceptions.  Nothing is kept between calls.
-#include <torch/csrc/autograd/python_variable.h>
-#include <c10/hip/HIPStream.h>
 #include <ATen/ops/empty.h>
 
 #include <type_traits>
 #include <utility>
 
 #include "../../include/bf16x_hip.h"
+#include "host_common.h"
 
 namespace {
-
-// An ordinary tensor (or Parameter), or null.
-const at::Tensor* tensor_of(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 bool on_gpu(const at::Tensor& t, int device) {
   return t.layout() == c10::kStrided && t.is_cuda() && t.get_device() == device && t.is_contiguous();
@@ -45,16 +42,6 @@ int weight_device(PyObject* const* o) {
 int32_t x_code(c10::ScalarType t) {
   return t == c10::kBFloat16 ? BF16X_BF16 : t == c10::kHalf ? BF16X_F16 : t == c10::kFloat ? BF16X_F32 : -1;
 }
-
-// The GIL given up for the scope (and taken again when an exception leaves it):
-// a launch or an allocation may wait for the GPU, and a host callback that the
-// GPU waits for may need Python.
-struct WithoutGil {
-  PyThreadState* state = PyEval_SaveThread();
-  ~WithoutGil() { PyEval_RestoreThread(state); }
-};
-
-void* stream_of(int dev) { return (void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream(); }
 
 // gemv(x, sign, mant, delta, emax, tile_off, tile_ent, tile_sat, out_f, in_f,
 // sub, out): y; None when the Python path has to take the call; the status (an
@@ -203,4 +190,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddFunctions(m, bf16x_serve_methods) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

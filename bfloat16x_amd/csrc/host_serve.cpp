@@ -1,0 +1,354 @@
+// Serving operators of the CPython module _host: the checks, the outputs and
+// workspaces, and the launches of kv4.append, kv4.read, kv4.attention and
+// sampling.sample.  A decode step calls them once per layer and token, with
+// kernels of a few microseconds, so the whole host path is native; there is no
+// second one in Python.  What a kernel could not take as it is (a type, a shape, a
+// device) raises TypeError or ValueError, before anything that touches the GPU;
+// the status of the C entry is returned for _lib.check.
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+
+#include <cmath>
+#include <initializer_list>
+#include <utility>
+#include <vector>
+
+#include "../../include/bf16x_llama.h"
+#include "host_common.h"
+
+namespace {
+
+struct Refused {};                         // a Python error is set
+
+[[noreturn]] void refuse(PyObject* kind, const char* format, const char* name, const char* what = "") {
+  PyErr_Format(kind, format, name, what);
+  throw Refused{};
+}
+
+const at::Tensor& need_tensor(PyObject* o, const char* name) {
+  const at::Tensor* t = tensor_of(o);
+  if (!t || t->layout() != c10::kStrided) refuse(PyExc_TypeError, "%s must be a tensor", name);
+  return *t;
+}
+const at::Tensor& need(PyObject* o, const char* name, c10::ScalarType type) {
+  const at::Tensor& t = need_tensor(o, name);
+  if (t.scalar_type() != type) refuse(PyExc_TypeError, "%s must be %s", name, c10::toString(type));
+  return t;
+}
+const at::Tensor* maybe(PyObject* o, const char* name, c10::ScalarType type) {
+  return o == Py_None ? nullptr : &need(o, name, type);
+}
+
+int32_t type_code(const at::Tensor& t, const char* name, bool wide) {
+  const c10::ScalarType s = t.scalar_type();
+  if (s == c10::kBFloat16) return BF16X_BF16;
+  if (s == c10::kHalf) return BF16X_F16;
+  if (s == c10::kFloat && wide) return BF16X_F32;
+  refuse(PyExc_TypeError, "%s must be %s", name, wide ? "bf16, fp16 or fp32" : "bf16 or fp16");
+}
+
+int64_t integer(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw Refused{};
+  return v;
+}
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Refused{};
+  return v;
+}
+
+void one_gpu(std::initializer_list<std::pair<const at::Tensor*, const char*>> all) {
+  int dev = -1;
+  for (const auto& [t, name] : all) {
+    if (!t) continue;
+    if (!t->is_cuda()) refuse(PyExc_ValueError, "%s must be a GPU tensor", name);
+    if (dev < 0) dev = t->get_device();
+    if (t->get_device() != dev) refuse(PyExc_ValueError, "%s is on another GPU", name);
+  }
+}
+
+// [batch, tokens, heads, head_dim] rows a kernel reads by strides; copied where
+// a head is not contiguous or does not start at a multiple of 16 bytes.
+at::Tensor rows(const at::Tensor& t) {
+  const int64_t size = t.element_size();
+  bool ok = t.stride(3) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
+  for (int d = 0; d < 3; ++d) ok = ok && (t.size(d) == 1 || t.stride(d) * size % 16 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// (a stride that is never stepped over may be anything)
+int64_t step(const at::Tensor& t, int d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
+struct Cache {
+  const at::Tensor *kc, *ks, *vc, *vs;
+  int64_t batch, kv, max_len, dim;
+};
+Cache cache_of(PyObject* o) {
+  const bool tuple = PyTuple_Check(o);
+  if (!(tuple ? PyTuple_GET_SIZE(o) == 4 : PyList_Check(o) && PyList_GET_SIZE(o) == 4))
+    refuse(PyExc_TypeError, "%s must be the four tensors of a Kv4Cache (%s)", "cache", "k, k_scale, v, v_scale");
+  PyObject* a[4];
+  for (int i = 0; i < 4; ++i) a[i] = tuple ? PyTuple_GET_ITEM(o, i) : PyList_GET_ITEM(o, i);
+  Cache c;
+  c.kc = &need(a[0], "cache k", c10::kByte);
+  c.ks = &need(a[1], "cache k_scale", c10::kHalf);
+  c.vc = &need(a[2], "cache v", c10::kByte);
+  c.vs = &need(a[3], "cache v_scale", c10::kHalf);
+  if (c.kc->dim() != 4) refuse(PyExc_ValueError, "%s must be [batch, kv heads, max_len, head_dim / 2]", "cache k");
+  c.batch = c.kc->size(0);
+  c.kv = c.kc->size(1);
+  c.max_len = c.kc->size(2);
+  c.dim = 2 * c.kc->size(3);
+  if (c.dim != 64 && c.dim != 128) refuse(PyExc_ValueError, "%s: head_dim must be 64 or 128", "cache k");
+  if (c.kv < 1 || c.max_len < 1) refuse(PyExc_ValueError, "%s has no rows", "cache k");
+  if (c.vc->sizes() != c.kc->sizes()) refuse(PyExc_ValueError, "%s must have the shape of cache k", "cache v");
+  for (const at::Tensor* s : {c.ks, c.vs})
+    if (s->sizes() != at::IntArrayRef({c.batch, c.kv, c.max_len, c.dim / 32, 2}))
+      refuse(PyExc_ValueError, "%s must be [batch, kv heads, max_len, head_dim / 32, 2]", "cache k_scale and v_scale");
+  for (const at::Tensor* t : {c.kc, c.ks, c.vc, c.vs})
+    if (!t->is_contiguous()) refuse(PyExc_ValueError, "%s must be contiguous", "the cache's tensors");
+  return c;
+}
+
+// int32 [batch], contiguous
+const at::Tensor* per_sequence(const at::Tensor* t, const char* name, int64_t batch) {
+  if (t && (t->numel() != batch || !t->is_contiguous()))
+    refuse(PyExc_ValueError, "%s must be contiguous, one number per sequence", name);
+  return t;
+}
+
+void need_rows(const at::Tensor& t, const char* name, int64_t batch, int64_t tokens, int64_t heads, int64_t dim) {
+  if (t.dim() != 4 || t.size(0) != batch || (tokens >= 0 && t.size(1) != tokens) || (heads >= 0 && t.size(2) != heads) ||
+      t.size(3) != dim)
+    refuse(PyExc_ValueError, "%s must be [batch, tokens, heads, head_dim] of the cache's batch and head_dim%s", name,
+           heads >= 0 ? ", with its kv heads" : "");
+}
+
+template <class F>
+PyObject* guarded(F f) {
+  try {
+    return f();
+  } catch (const Refused&) {
+    return nullptr;
+  } catch (const std::exception& e) {
+    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+  }
+}
+
+void arity(Py_ssize_t n, Py_ssize_t want) {
+  if (n == want) return;
+  PyErr_Format(PyExc_TypeError, "%zd arguments expected", want);
+  throw Refused{};
+}
+
+// A result: the status where it is not 0, otherwise the tensors.
+PyObject* answer(int rc, std::vector<at::Tensor> out) {
+  if (rc != 0) return PyLong_FromLong(rc);
+  if (out.empty()) Py_RETURN_NONE;
+  if (out.size() == 1) return THPVariable_Wrap(std::move(out[0]));
+  PyObject* t = PyTuple_New((Py_ssize_t)out.size());
+  for (size_t i = 0; t && i < out.size(); ++i) {
+    PyObject* o = THPVariable_Wrap(std::move(out[i]));
+    if (!o) {
+      Py_DECREF(t);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(t, (Py_ssize_t)i, o);
+  }
+  return t;
+}
+
+void* data(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+void* data(const at::Tensor& t) { return t.data_ptr(); }
+
+// kv4_append(k, v, cache, pos, q, cos_sin): the rotated q, or None
+PyObject* kv4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arity(n, 6);
+    const Cache c = cache_of(a[2]);
+    const at::Tensor &k = need_tensor(a[0], "k"), &v = need_tensor(a[1], "v");
+    const int32_t type = type_code(k, "k", true);
+    if (v.scalar_type() != k.scalar_type()) refuse(PyExc_TypeError, "%s must have k's type", "v");
+    need_rows(k, "k", c.batch, -1, c.kv, c.dim);
+    const int64_t tokens = k.size(1);
+    need_rows(v, "v", c.batch, tokens, c.kv, c.dim);
+    const at::Tensor* pos = per_sequence(&need(a[3], "pos", c10::kInt), "pos", c.batch);
+    const at::Tensor* cs = maybe(a[5], "cos_sin", c10::kFloat);
+    const at::Tensor* q = nullptr;
+    if (a[4] != Py_None) {
+      q = &need_tensor(a[4], "q");
+      if (q->scalar_type() != k.scalar_type()) refuse(PyExc_TypeError, "%s must have k's type", "q");
+      need_rows(*q, "q", c.batch, tokens, -1, c.dim);
+      if (!cs) refuse(PyExc_ValueError, "%s is only rotated: it needs cos_sin", "q");
+    }
+    if (cs && (!cs->is_contiguous() || cs->dim() != 3 || cs->size(0) < 1 || cs->size(1) != c.dim / 2 ||
+               cs->size(2) != 2 || (uintptr_t)cs->data_ptr() % 16))
+      refuse(PyExc_ValueError, "%s must be contiguous fp32 [positions, head_dim / 2, 2]", "cos_sin");
+    one_gpu({{&k, "k"}, {&v, "v"}, {c.kc, "cache k"}, {c.ks, "cache k_scale"}, {c.vc, "cache v"},
+             {c.vs, "cache v_scale"}, {pos, "pos"}, {cs, "cos_sin"}, {q, "q"}});
+    at::Tensor out;
+    int rc = 0;
+    {
+      const WithoutGil no_gil;
+      const c10::DeviceGuard guard(k.device());
+      const at::Tensor kk = rows(k), vv = rows(v), qq = q ? rows(*q) : at::Tensor();
+      if (q) out = at::empty({c.batch, tokens, q->size(2), c.dim}, q->options());
+      if (k.numel() > 0)
+        rc = bf16x_kv4_append(q ? data(qq) : nullptr, q ? step(qq, 0) : 0, q ? step(qq, 1) : 0, q ? step(qq, 2) : 0,
+                            data(kk), step(kk, 0), step(kk, 1), step(kk, 2), data(vv), step(vv, 0), step(vv, 1),
+                            step(vv, 2), type, c.batch, tokens, q ? q->size(2) : 0, c.kv, c.dim, c.max_len,
+                            (const int32_t*)data(pos), (const float*)data(cs), cs ? cs->size(0) : 0,
+                            q ? data(out) : nullptr, (uint8_t*)data(c.kc), (uint16_t*)data(c.ks), (uint8_t*)data(c.vc),
+                            (uint16_t*)data(c.vs), stream_of(k.get_device()));
+    }
+    return q ? answer(rc, {out}) : answer(rc, {});
+  });
+}
+
+// kv4_read(cache, pos, tokens, like): (k, v) in like's type
+PyObject* kv4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arity(n, 4);
+    const Cache c = cache_of(a[0]);
+    const at::Tensor* pos = per_sequence(&need(a[1], "pos", c10::kInt), "pos", c.batch);
+    const int64_t tokens = integer(a[2]);
+    if (tokens < 0) refuse(PyExc_ValueError, "%s must not be negative", "tokens");
+    const int64_t code = integer(a[3]);
+    const c10::ScalarType type = code == BF16X_BF16 ? c10::kBFloat16 : code == BF16X_F16 ? c10::kHalf : c10::kFloat;
+    one_gpu({{c.kc, "cache k"}, {c.ks, "cache k_scale"}, {c.vc, "cache v"}, {c.vs, "cache v_scale"}, {pos, "pos"}});
+    at::Tensor k, v;
+    int rc;
+    {
+      const WithoutGil no_gil;
+      const c10::DeviceGuard guard(c.kc->device());
+      k = at::empty({c.batch, tokens, c.kv, c.dim}, c.kc->options().dtype(type));
+      v = at::empty({c.batch, tokens, c.kv, c.dim}, c.kc->options().dtype(type));
+      rc = k.numel() == 0 ? 0
+                          : bf16x_kv4_read((const uint8_t*)data(c.kc), (const uint16_t*)data(c.ks),
+                                           (const uint8_t*)data(c.vc), (const uint16_t*)data(c.vs), c.batch, tokens, c.kv,
+                                           c.dim, c.max_len, (const int32_t*)data(pos), (int32_t)code, data(k), data(v),
+                                           stream_of(c.kc->get_device()));
+    }
+    return answer(rc, {k, v});
+  });
+}
+
+// kv4_attention(q, cache, pos, start, window, scale, out): out
+PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arity(n, 7);
+    const Cache c = cache_of(a[1]);
+    const at::Tensor& q = need_tensor(a[0], "q");
+    const int32_t type = type_code(q, "q", false);
+    need_rows(q, "q", c.batch, -1, -1, c.dim);
+    const int64_t tokens = q.size(1), heads = q.size(2);
+    if (heads < 1 || heads % c.kv) refuse(PyExc_ValueError, "%s: the cache's kv heads must divide its heads", "q");
+    const at::Tensor* pos = per_sequence(&need(a[2], "pos", c10::kInt), "pos", c.batch);
+    const at::Tensor* start = per_sequence(maybe(a[3], "start", c10::kInt), "start", c.batch);
+    const int64_t window = integer(a[4]);
+    if (window < 0) refuse(PyExc_ValueError, "%s must not be negative", "window");
+    const double scale = a[5] == Py_None ? 1.0 / std::sqrt((double)c.dim) : number(a[5]);
+    const at::Tensor* given = nullptr;
+    if (a[6] != Py_None) {
+      given = &need(a[6], "out", q.scalar_type());
+      if (!given->is_contiguous() || given->sizes() != q.sizes())
+        refuse(PyExc_ValueError, "%s must be contiguous, of q's shape", "out");
+    }
+    one_gpu({{&q, "q"}, {c.kc, "cache k"}, {c.ks, "cache k_scale"}, {c.vc, "cache v"}, {c.vs, "cache v_scale"},
+             {pos, "pos"}, {start, "start"}, {given, "out"}});
+    at::Tensor out;
+    int rc = 0;
+    {
+      const WithoutGil no_gil;
+      const c10::DeviceGuard guard(q.device());
+      const at::Tensor qq = rows(q);
+      out = given ? *given : at::empty(q.sizes(), q.options());
+      if (out.numel() > 0) {
+        const int64_t bytes = bf16x_kv4_attention_workspace(c.batch, tokens, heads, c.kv, c.dim, c.max_len);
+        const at::Tensor ws = bytes > 0 ? at::empty({bytes}, c.kc->options()) : at::Tensor();
+        rc = bf16x_kv4_attention(data(qq), step(qq, 0), step(qq, 1), step(qq, 2), type, c.batch, tokens, heads, c.kv,
+                                 c.dim, c.max_len, (const uint8_t*)data(c.kc), (const uint16_t*)data(c.ks),
+                                 (const uint8_t*)data(c.vc), (const uint16_t*)data(c.vs), (const int32_t*)data(pos),
+                                 (const int32_t*)data(start), window, (float)scale, data(out),
+                                 ws.defined() ? data(ws) : nullptr, bytes > 0 ? bytes : 0, stream_of(q.get_device()));
+      }
+    }
+    return answer(rc, {out});
+  });
+}
+
+// One setting: a number for all rows, or a tensor of one per row.
+template <class T>
+const T* setting(PyObject* o, const char* name, c10::ScalarType type, int64_t rows, T& all, const at::Tensor*& kept) {
+  if (!THPVariable_Check(o)) {
+    all = std::is_same<T, float>::value
+              ? (T)number(o)
+              : (T)std::min<int64_t>(std::max<int64_t>(integer(o), 0), 0x7FFFFFFF);
+    return nullptr;
+  }
+  kept = &need(o, name, type);
+  if (kept->numel() != rows || !kept->is_contiguous())
+    refuse(PyExc_ValueError, "%s must be contiguous, one number per row", name);
+  return (const T*)kept->data_ptr();
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p, token, state, history): (token, logprob)
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arity(n, 9);
+    const at::Tensor& logits = need_tensor(a[0], "logits");
+    const int32_t type = type_code(logits, "logits", true);
+    if (logits.dim() != 1 && logits.dim() != 2) refuse(PyExc_ValueError, "%s must be [rows, vocab] or [vocab]", "logits");
+    const int64_t nrows = logits.dim() == 2 ? logits.size(0) : 1, vocab = logits.size(-1);
+    if (vocab < 1 || vocab > (1 << 20) || nrows > 65535)
+      refuse(PyExc_ValueError, "%s must have 1 to 1048576 columns and at most 65535 rows", "logits");
+    const at::Tensor& u = need(a[1], "u", c10::kFloat);
+    const at::Tensor* state = maybe(a[7], "state", c10::kInt);
+    const at::Tensor* history = maybe(a[8], "history", c10::kInt);
+    if (!u.is_contiguous()) refuse(PyExc_ValueError, "%s must be contiguous", "u");
+    if (state) {
+      if (nrows != 1 || state->numel() < 2 || !state->is_contiguous() || u.numel() < 1)
+        refuse(PyExc_ValueError, "%s goes with one row, at least one number in u, and is int32 [2]", "state");
+    } else if (u.numel() != nrows) {
+      refuse(PyExc_ValueError, "%s must hold one number per row", "u");
+    }
+    if (history && (!state || !history->is_contiguous()))
+      refuse(PyExc_ValueError, "%s must be contiguous and goes with state", "history");
+    bf16x_sample_settings s{};
+    const at::Tensor *tt = nullptr, *tk = nullptr, *tp = nullptr, *tm = nullptr;
+    s.temperature = setting(a[2], "temperature", c10::kFloat, nrows, s.temperature_all, tt);
+    s.top_k = setting(a[3], "top_k", c10::kInt, nrows, s.top_k_all, tk);
+    s.top_p = setting(a[4], "top_p", c10::kFloat, nrows, s.top_p_all, tp);
+    s.min_p = setting(a[5], "min_p", c10::kFloat, nrows, s.min_p_all, tm);
+    const at::Tensor* given = maybe(a[6], "token", c10::kLong);
+    if (given && (given->numel() < nrows || !given->is_contiguous()))
+      refuse(PyExc_ValueError, "%s must be contiguous, one number per row", "token");
+    one_gpu({{&logits, "logits"}, {&u, "u"}, {tt, "temperature"}, {tk, "top_k"}, {tp, "top_p"}, {tm, "min_p"},
+             {given, "token"}, {state, "state"}, {history, "history"}});
+    at::Tensor token, logprob;
+    int rc = 0;
+    {
+      const WithoutGil no_gil;
+      const c10::DeviceGuard guard(logits.device());
+      const at::Tensor x = logits.stride(-1) == 1 || vocab == 1 ? logits : logits.clone(at::MemoryFormat::Contiguous);
+      token = given ? *given : at::empty({nrows}, logits.options().dtype(c10::kLong));
+      logprob = at::empty({nrows}, logits.options().dtype(c10::kFloat));
+      if (nrows > 0) {
+        const int64_t bytes = bf16x_sample_workspace(nrows, vocab);
+        const at::Tensor ws = at::empty({bytes}, logits.options().dtype(c10::kByte));
+        rc = bf16x_sample(data(x), type, x.dim() == 2 && nrows > 1 ? x.stride(0) : 0, nrows, vocab,
+                          (const float*)data(u), u.numel(), &s, (int64_t*)data(token), (float*)data(logprob),
+                          (int32_t*)data(state), (int32_t*)data(history), history ? history->numel() : 0, data(ws), bytes,
+                          stream_of(logits.get_device()));
+      }
+    }
+    return answer(rc, {token, logprob});
+  });
+}
+
+#define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
+
+}  // namespace
+
+PyMethodDef bf16x_serve_methods[] = {FAST(kv4_append), FAST(kv4_read), FAST(kv4_attention), FAST(sample),
+                                     {nullptr, nullptr, 0, nullptr}};

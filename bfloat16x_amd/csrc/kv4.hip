@@ -1,0 +1,651 @@
+// The 4-bit KV cache (include/bf16x_llama.h): append, read, attention.
+//
+// A cache row of a head (128 values: 64 bytes of codes, 16 of scales) is read
+// as it is needed by the 16x16x32 MFMA, whose operands hold 8 consecutive
+// values of the contraction axis per lane (lane l, c = l % 16, g = l / 16:
+// A[c][8 g + e], B[8 g + e][c], D register v = D[4 g + v][c]):
+//  * S^T = K Q^T contracts over head_dim: a lane's 8 values are one word of
+//    codes of one key, and which 8 of the dims form a step is free as long as
+//    q is read in the same order;
+//  * O^T = V^T P^T contracts over keys: the scores come out of the first
+//    product with 4 g + v as the key, so slot 8 g + e of a 32-key step stands
+//    for key 4 g + e (e < 4) or 16 + 4 g + e - 4, and a lane's weights are its
+//    own scores.  V's operand needs 8 keys of one dim: the codes of two keys
+//    are interleaved byte by byte (v_perm_b32) before they become numbers.
+// A code c becomes the fp16 number minimum + scale c with three packed
+// operations for two codes: the nibbles are put under the exponent at which
+// their lowest bit counts 1 (v_and_or_b32: 1024 + c, or 64 + c for a high
+// nibble), the 1024 or 64 is taken off, and one fma rounds once.
+#include "bf16x_device.h"
+#include "launch_common.h"
+#include "../../include/bf16x_llama.h"
+
+namespace {
+using namespace bf16x;
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLargest = 61440.f;       // 15 x 4096: minimum + 15 scale stays an fp16 number whatever was rounded
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
+__device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// Codes of the low nibbles of bytes 0 and 2, or of their high nibbles.
+__device__ __forceinline__ h2 low_codes(uint32_t w) { return as_h2((w & 0x000F000Fu) | 0x64006400u) - h2{1024, 1024}; }
+__device__ __forceinline__ h2 high_codes(uint32_t w) { return as_h2((w & 0x00F000F0u) | 0x54005400u) - h2{64, 64}; }
+
+// The 8 values of a word of codes, in order; s = (scale, scale), m = (minimum, minimum).
+__device__ __forceinline__ h8 word_values(uint32_t w, h2 s, h2 m) {
+  const h2 a = __builtin_elementwise_fma(low_codes(w), s, m), b = __builtin_elementwise_fma(high_codes(w), s, m);
+  w >>= 8;
+  const h2 c = __builtin_elementwise_fma(low_codes(w), s, m), d = __builtin_elementwise_fma(high_codes(w), s, m);
+  return __builtin_bit_cast(h8, u32x4{as_u32(a), as_u32(b), as_u32(c), as_u32(d)});
+}
+// (scale, scale) and (minimum, minimum) of a scale word.
+__device__ __forceinline__ h2 scale_of(uint32_t w) { return as_h2(__builtin_amdgcn_perm(w, w, 0x01000100u)); }
+__device__ __forceinline__ h2 minimum_of(uint32_t w) { return as_h2(__builtin_amdgcn_perm(w, w, 0x03020302u)); }
+
+// ---------------------------------------------------------------------------
+// Append and read.  8 values per lane (one word of codes), so D / 8 lanes per
+// row; the 4 lanes of a group meet in two quad exchanges.
+
+template <int TYPE>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&x)[8]) {
+  if constexpr (TYPE == BF16X_F32) {
+    const f4 a = *(const f4*)((const float*)p + i), b = *(const f4*)((const float*)p + i + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
+  } else {
+    const u32x4 r = *(const u32x4*)((const uint16_t*)p + i);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (TYPE == BF16X_BF16) {
+        x[2 * e] = bf16lo_to_f32(w[e]);
+        x[2 * e + 1] = bf16hi_to_f32(w[e]);
+      } else {
+        const h2 h = as_h2(w[e]);
+        x[2 * e] = (float)h.x;
+        x[2 * e + 1] = (float)h.y;
+      }
+    }
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (TYPE == BF16X_BF16) return f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16);
+  return as_u32(h2{(_Float16)a, (_Float16)b});
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&x)[8]) {
+  if constexpr (TYPE == BF16X_F32) {
+    *(f4*)((float*)p + i) = f4{x[0], x[1], x[2], x[3]};
+    *(f4*)((float*)p + i + 4) = f4{x[4], x[5], x[6], x[7]};
+  } else {
+    *(u32x4*)((uint16_t*)p + i) = u32x4{pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3]), pack2<TYPE>(x[4], x[5]),
+                                        pack2<TYPE>(x[6], x[7])};
+  }
+}
+
+struct AppendArgs {
+  const void *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  int64_t rows;                            // batch x tokens x heads of a token
+  int tokens, H, KV, max_len;
+  const int32_t* pos;
+  const float* cos_sin;
+  int64_t cos_rows;
+  void* q_out;
+  uint32_t *kc, *ks, *vc, *vs;
+};
+
+template <int D, int TYPE>
+__global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
+#pragma clang fp contract(off)             // the rotation's products are rounded one by one, as its definition says
+  constexpr int LR = D / 8;                // lanes per row
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;
+  const int l = threadIdx.x % LR;
+  if (row >= a.rows) return;               // whole rows: the lanes of a group leave together
+  const int heads = a.H + 2 * a.KV;
+  const int64_t bt = row / heads;
+  const int h = (int)(row - bt * heads), b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
+  const int64_t p = (int64_t)a.pos[b] + t;
+  const bool is_q = h < a.H, is_k = !is_q && h < a.H + a.KV;
+  const int hk = is_q ? h : is_k ? h - a.H : h - a.H - a.KV;
+  if (!is_q && (p < 0 || p >= a.max_len)) return;
+  const void* src = is_q ? a.q : is_k ? a.k : a.v;
+  const int64_t off = is_q ? b * a.q_sb + t * a.q_st + hk * a.q_sh
+                           : is_k ? b * a.k_sb + t * a.k_st + hk * a.k_sh : b * a.v_sb + t * a.v_st + hk * a.v_sh;
+  float x[8];
+  load8<TYPE>(src, off + 8 * l, x);
+  if (a.cos_sin && (is_q || is_k)) {
+    float y[8];
+    load8<TYPE>(src, off + 8 * (l ^ (LR / 2)), y);
+    const int64_t pc = p < 0 ? 0 : p >= a.cos_rows ? a.cos_rows - 1 : p;
+    const f4* cs = (const f4*)(a.cos_sin + (pc * (D / 2) + 8 * (l % (LR / 2))) * 2);
+    const bool upper = l >= LR / 2;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f4 c = cs[e];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float own = x[2 * e + u] * c[2 * u], other = y[2 * e + u] * c[2 * u + 1];
+        x[2 * e + u] = upper ? own + other : own - other;
+      }
+    }
+  }
+  if (is_q) {
+    store8<TYPE>(a.q_out, (bt * a.H + hk) * D + 8 * l, x);
+    return;
+  }
+  float mn = kLargest, mx = -kLargest;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = x[e] != x[e] ? 0.f : fminf(fmaxf(x[e], -kLargest), kLargest);
+    mn = fminf(mn, x[e]);
+    mx = fmaxf(mx, x[e]);
+  }
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    mn = fminf(mn, __shfl_xor(mn, o, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  }
+  const _Float16 low = (_Float16)mn;
+  const float lowf = (float)low;
+  const _Float16 sc = (_Float16)(fmaxf(mx - lowf, 0.f) / 15.f);
+  const float scf = (float)sc;
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float n = scf > 0.f ? fminf(fmaxf(__builtin_rintf((x[e] - lowf) / scf), 0.f), 15.f) : 0.f;
+    w |= (uint32_t)n << (e & 1 ? 14 + 2 * e : 2 * e);
+  }
+  const int64_t out = ((int64_t)b * a.KV + hk) * a.max_len + p;
+  (is_k ? a.kc : a.vc)[out * LR + l] = w;
+  if ((l & 3) == 0) (is_k ? a.ks : a.vs)[out * (D / 32) + l / 4] = as_u32(h2{sc, low});
+}
+
+struct ReadArgs {
+  const uint32_t *kc, *ks, *vc, *vs;
+  int64_t rows;                            // 2 x batch x tokens x KV
+  int tokens, KV, max_len;
+  const int32_t* pos;
+  void *k_out, *v_out;
+};
+
+template <int D, int TYPE>
+__global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
+  constexpr int LR = D / 8;
+  int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;
+  const int l = threadIdx.x % LR;
+  if (row >= a.rows) return;
+  const bool is_k = row < a.rows / 2;
+  if (!is_k) row -= a.rows / 2;
+  const int64_t bt = row / a.KV;
+  const int h = (int)(row - bt * a.KV), b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
+  const int64_t p = (int64_t)a.pos[b] + t;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (p >= 0 && p < a.max_len) {
+    const int64_t at = ((int64_t)b * a.KV + h) * a.max_len + p;
+    const uint32_t w = (is_k ? a.kc : a.vc)[at * LR + l];
+    const h2 s = as_h2((is_k ? a.ks : a.vs)[at * (D / 32) + l / 4]);
+    const float sc = (float)s.x, low = (float)s.y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf(sc, (float)((w >> (e & 1 ? 14 + 2 * e : 2 * e)) & 15u), low);
+  }
+  store8<TYPE>(is_k ? a.k_out : a.v_out, row * D + 8 * l, x);
+}
+
+// ---------------------------------------------------------------------------
+// Attention
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t q_sb, q_st, q_sh;
+  int batch, tokens, H, KV, G, max_len;
+  int rows;                                // tokens x G: query rows of a KV head, row t G + g
+  int tiles, splits;
+  int window;                              // 0: none
+  float scale;
+  const uint8_t* kc;
+  const uint32_t* ks;
+  const uint8_t* vc;
+  const uint32_t* vs;
+  const int32_t *pos, *start;
+  uint16_t* out;
+  float* part;                             // [splits][batch KV rows][D] unnormalised outputs, then [..][2] (max, sum)
+};
+
+// Keys [lo, hi) that the query at token t sees.
+__device__ __forceinline__ void key_range(const AttnArgs& a, int b, int t, int& lo, int& hi) {
+  const int64_t p = (int64_t)a.pos[b] + t;
+  const int64_t n = p + 1 < 0 ? 0 : p + 1 > a.max_len ? a.max_len : p + 1;
+  int64_t f = a.start ? a.start[b] : 0;
+  if (a.window && p + 1 - a.window > f) f = p + 1 - a.window;
+  f = f < 0 ? 0 : f;
+  hi = (int)n;
+  lo = (int)(f < n ? f : n);
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t out2(float a, float b) {
+  return BF ? f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16) : as_u32(h2{(_Float16)a, (_Float16)b});
+}
+
+// The query operand of a lane: NW words of 2 values at `src` brought to fp16
+// by the power of two that puts the row's largest value (over the 4 lanes of
+// the row) into [1, 2); returns its inverse.  Exact for every value within
+// 2^-14 of the row's largest.
+template <bool BF, int N>
+__device__ __forceinline__ float load_query(const uint16_t* src, bool valid, h8 (&qb)[N], const int (&off)[N]) {
+  float x[N][8];
+  float mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+    if (valid) load8<BF ? BF16X_BF16 : BF16X_F16>(src, off[i], x[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
+  }
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  int e2 = (int)(__float_as_uint(mx) >> 23) - 127;
+  e2 = mx > 0.f && e2 < 128 ? max(e2, -100) : 0;
+  const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qb[i][e] = (_Float16)(x[i][e] * down);
+  return __uint_as_float((uint32_t)(127 + e2) << 23);
+}
+
+// Few query rows (single tokens, drafts): a tile of 16 rows; 4 waves take the
+// 32-key steps of the workgroup's range in turn, each straight from the cache
+// into MFMA operands, with a running maximum and sum per row; the waves meet
+// in LDS once, at the end.
+template <int D>
+struct Step {
+  static constexpr int W = D / 32;         // words of codes of a key per lane in the first product
+  uint32_t kc[2][W], ks[2], vc[8], vs[8];
+};
+
+template <int D>
+__device__ __forceinline__ void load_step(Step<D>& s, const uint8_t* kc, const uint32_t* ks, const uint8_t* vc,
+                                          const uint32_t* vs, int j0, int last, int c, int g) {
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const int64_t j = min(j0 + 16 * kt + c, last);
+    if constexpr (D == 128) {
+      const u32x4 w = *(const u32x4*)(kc + j * (D / 2) + 16 * g);
+      s.kc[kt][0] = w.x, s.kc[kt][1] = w.y, s.kc[kt][2] = w.z, s.kc[kt][3] = w.w;
+      s.ks[kt] = ks[j * (D / 32) + g];
+    } else {
+      const uint2 w = *(const uint2*)(kc + j * (D / 2) + 8 * g);
+      s.kc[kt][0] = w.x, s.kc[kt][1] = w.y;
+      s.ks[kt] = ks[j * (D / 32) + (g >> 1)];
+    }
+  }
+  const int dw = c & (D / 8 - 1);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int64_t j = min(j0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4), last);
+    s.vc[e] = *(const uint32_t*)(vc + j * (D / 2) + 4 * dw);
+    s.vs[e] = vs[j * (D / 32) + dw / 4];
+  }
+}
+
+constexpr int kRowWaves = 4;
+
+template <int D, bool BF>
+__global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs a) {
+  constexpr int W = D / 32, NT = D / 16;   // steps of the first product, row blocks of the second
+  __shared__ float lo_[kRowWaves][16][D + 4];
+  __shared__ float lm[kRowWaves][16], ll[kRowWaves][16];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int id = blockIdx.x;
+  const int sp = id % a.splits;
+  id /= a.splits;
+  const int tile = id % a.tiles;
+  id /= a.tiles;
+  const int kvh = id % a.KV, b = id / a.KV;
+  const int r = 16 * tile + c;             // this lane's query row
+  const bool valid = r < a.rows;
+  const int t = min(r, a.rows - 1) / a.G, hg = min(r, a.rows - 1) - t * a.G;
+  int lo, hi, LO, HI, unused;
+  key_range(a, b, t, lo, hi);
+  key_range(a, b, 16 * tile / a.G, LO, unused);
+  key_range(a, b, min(16 * tile + 15, a.rows - 1) / a.G, unused, HI);
+  const int base = LO & ~31;
+  const int steps = HI > LO ? (HI - base + 31) >> 5 : 0;
+  const int per = (steps + a.splits - 1) / a.splits;
+  const int s1 = min((sp + 1) * per, steps);
+
+  const int64_t head = ((int64_t)b * a.KV + kvh) * a.max_len;
+  const uint8_t *kc = a.kc + head * (D / 2), *vc = a.vc + head * (D / 2);
+  const uint32_t *ks = a.ks + head * (D / 32), *vs = a.vs + head * (D / 32);
+
+  h8 qb[W];
+  int qoff[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) qoff[i] = g * (D / 4) + 8 * i;
+  const float back = load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, valid, qb, qoff);
+  const float sc = a.scale * kLog2e * back;
+
+  float m = -INFINITY, l = 0.f;
+  f4 o[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
+
+  Step<D> cur, next;
+  int s = sp * per + w;
+  if (s < s1) load_step<D>(cur, kc, ks, vc, vs, base + 32 * s, a.max_len - 1, c, g);
+  for (; s < s1; s += kRowWaves) {
+    if (s + kRowWaves < s1)
+      load_step<D>(next, kc, ks, vc, vs, base + 32 * (s + kRowWaves), a.max_len - 1, c, g);
+    const int j0 = base + 32 * s;
+    // scores of keys j0 + 16 kt + 4 g + v for row c
+    float x[8];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const h2 sc2 = scale_of(cur.ks[kt]), mn2 = minimum_of(cur.ks[kt]);
+      f4 acc = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_values(cur.kc[kt][i], sc2, mn2), qb[i], acc, 0, 0, 0);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int j = j0 + 16 * kt + 4 * g + v;
+        x[4 * kt + v] = j >= lo && j < hi ? acc[v] * sc : -INFINITY;
+      }
+    }
+    float mb = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
+    mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+    const float mn = fmaxf(m, mb);
+    const float from = mn == -INFINITY ? 0.f : mn;               // no key seen yet: every weight is 0
+    const float alpha = __builtin_amdgcn_exp2f(m - from);
+    m = mn;
+    float ps = 0.f;
+    h8 pb;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float e = __builtin_amdgcn_exp2f(x[k] - from);
+      ps += e;
+      pb[k] = (_Float16)e;
+    }
+    l = l * alpha + ps;
+    // O^T += V^T P^T; keys that no row of the tile sees have value 0
+    uint32_t vsm[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = j0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+      vsm[e] = j >= LO && j < HI ? cur.vs[e] : 0u;
+    }
+    u32x4 av[NT];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const h2 s2 = as_h2(__builtin_amdgcn_perm(vsm[2 * k + 1], vsm[2 * k], 0x05040100u));
+      const h2 m2 = as_h2(__builtin_amdgcn_perm(vsm[2 * k + 1], vsm[2 * k], 0x07060302u));
+      uint32_t va = cur.vc[2 * k], vb = cur.vc[2 * k + 1];
+      if constexpr (D == 64) {             // lanes 8 .. 15 take the upper nibbles of the same words
+        va = c & 8 ? va >> 16 : va;
+        vb = c & 8 ? vb >> 16 : vb;
+      }
+#pragma unroll
+      for (int y = 0; y < NT / 2; ++y) {
+        const uint32_t two = __builtin_amdgcn_perm(vb, va, 0x0C040C00u + 0x00010001u * y);
+        av[2 * y][k] = as_u32(__builtin_elementwise_fma(low_codes(two), s2, m2));
+        av[2 * y + 1][k] = as_u32(__builtin_elementwise_fma(high_codes(two), s2, m2));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      o[n] *= alpha;
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, av[n]), pb, o[n], 0, 0, 0);
+    }
+    cur = next;
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+
+  // the waves' results meet: row c, dims of D row 4 g + v and row block n
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int rr = 4 * g + v;
+      // nibble n (upper nibbles for rows 8 .. 15 where D is 64) of a word: value 2 n below 4, else 2 n - 7
+      const int nib = D == 128 ? n : n + 4 * (rr >> 3);
+      const int dim = 8 * (D == 128 ? rr : rr & 7) + (nib < 4 ? 2 * nib : 2 * nib - 7);
+      lo_[w][c][dim] = o[n][v];
+    }
+  if (g == 0) lm[w][c] = m, ll[w][c] = l;
+  __syncthreads();
+  constexpr int E = 16 * D / (64 * kRowWaves);                  // values of the tile per thread
+  const int rr = tid / (D / E), d0 = tid % (D / E) * E;
+  const int R = 16 * tile + rr;
+  if (R >= a.rows) return;
+  float M = lm[0][rr];
+#pragma unroll
+  for (int u = 1; u < kRowWaves; ++u) M = fmaxf(M, lm[u][rr]);
+  float L = 0.f, y[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = 0.f;
+#pragma unroll
+  for (int u = 0; u < kRowWaves; ++u) {
+    const float f = lm[u][rr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lm[u][rr] - M);
+    L = fmaf(ll[u][rr], f, L);
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = fmaf(lo_[u][rr][d0 + e], f, y[e]);
+  }
+  if (a.splits == 1) {
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const int tt = R / a.G, hh = R - tt * a.G;
+    uint32_t* op = (uint32_t*)(a.out + (((int64_t)b * a.tokens + tt) * a.H + kvh * a.G + hh) * D + d0);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) op[e / 2] = out2<BF>(y[e] * inv, y[e + 1] * inv);
+    return;
+  }
+  const int64_t all = (int64_t)a.batch * a.KV * a.rows;
+  const int64_t at = sp * all + ((int64_t)b * a.KV + kvh) * a.rows + R;
+#pragma unroll
+  for (int e = 0; e < E; ++e) a.part[at * D + d0 + e] = y[e];
+  if (d0 == 0) {
+    float* ml = a.part + a.splits * all * D + 2 * at;
+    ml[0] = M;
+    ml[1] = L;
+  }
+}
+
+// Joins the splits of a row: one workgroup of D threads per row.
+template <int D, bool BF>
+__global__ __launch_bounds__(D) void kv4_attn_join_kernel(AttnArgs a) {
+  const int64_t all = (int64_t)a.batch * a.KV * a.rows, at = blockIdx.x;
+  const int d = threadIdx.x;
+  const float* ml = a.part + a.splits * all * D;
+  float M = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[2 * (s * all + at)]);
+  const float from = M == -INFINITY ? 0.f : M;
+  float L = 0.f, y = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t i = s * all + at;
+    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - from);
+    L = fmaf(ml[2 * i + 1], f, L);
+    y = fmaf(a.part[i * D + d], f, y);
+  }
+  const int64_t bk = at / a.rows;
+  const int r = (int)(at - bk * a.rows), t = r / a.G, hg = r - t * a.G;
+  const int64_t b = bk / a.KV;
+  const int kvh = (int)(bk - b * a.KV);
+  const float v = y * (L > 0.f ? 1.f / L : 0.f);
+  a.out[((b * a.tokens + t) * a.H + kvh * a.G + hg) * D + d] =
+      BF ? (uint16_t)f32_to_bf16_rne(v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+
+bool is_half(int32_t type) { return type == BF16X_BF16 || type == BF16X_F16; }
+
+int check_cache(int64_t batch, int64_t tokens, int64_t KV, int64_t D, int64_t max_len) {
+  if (D != 64 && D != 128) return BF16X_ESHAPE;
+  if (batch < 0 || tokens < 0) return BF16X_EARG;
+  if (KV <= 0 || KV > 65535 || max_len <= 0 || max_len > ((int64_t)1 << 30) || batch > ((int64_t)1 << 24) ||
+      tokens > ((int64_t)1 << 24))
+    return BF16X_ESHAPE;
+  return BF16X_OK;
+}
+
+// heads start at 16-byte multiples: base and strides (in elements of `size` bytes)
+bool rows_aligned(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t size) {
+  return aligned16(p) && sb * size % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
+}
+
+// How the work of an attention call is cut: tiles of 16 query rows, and splits
+// of their keys so that a small call still fills the card.
+struct Cut {
+  int tiles, splits;
+};
+Cut cut_of(int64_t batch, int64_t rows, int64_t KV, int64_t max_len) {
+  const int64_t tiles = (rows + 15) / 16, wgs = batch * KV * tiles;
+  const int64_t want = wgs > 0 ? 512 / wgs : 1, most = (max_len + 32 * kRowWaves - 1) / (32 * kRowWaves);
+  return {(int)tiles, (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 128}))};
+}
+
+}  // namespace
+
+extern "C" int bf16x_kv4_append(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
+                                int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                                int32_t type, int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                                int64_t head_dim, int64_t max_len, const int32_t* pos, const float* cos_sin,
+                                int64_t cos_rows, void* q_out, uint8_t* k_codes, uint16_t* k_scales, uint8_t* v_codes,
+                                uint16_t* v_scales, bf16x_stream_t stream) {
+  if (!k || !v || !pos || !k_codes || !k_scales || !v_codes || !v_scales) return BF16X_EARG;
+  if ((q != nullptr) != (q_out != nullptr) || (q && !cos_sin) || (cos_sin && cos_rows <= 0)) return BF16X_EARG;
+  if (type != BF16X_BF16 && type != BF16X_F16 && type != BF16X_F32) return BF16X_EDTYPE;
+  const int bad = check_cache(batch, tokens, n_kv_heads, head_dim, max_len);
+  if (bad) return bad;
+  if (q && (n_heads <= 0 || n_heads > 65535)) return BF16X_ESHAPE;
+  const int64_t size = type == BF16X_F32 ? 4 : 2;
+  if (!rows_aligned(k, k_sb, k_st, k_sh, size) || !rows_aligned(v, v_sb, v_st, v_sh, size) || !aligned4(pos) ||
+      (cos_sin && !aligned16(cos_sin)) || !aligned4(k_codes) || !aligned4(k_scales) || !aligned4(v_codes) ||
+      !aligned4(v_scales) || (q && (!rows_aligned(q, q_sb, q_st, q_sh, size) || !aligned16(q_out))))
+    return BF16X_EARG;
+  if (batch == 0 || tokens == 0) return BF16X_OK;
+  const int H = q ? (int)n_heads : 0;
+  AppendArgs a{q, k, v, q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, batch * tokens * (H + 2 * n_kv_heads),
+               (int)tokens, H, (int)n_kv_heads, (int)max_len, pos, cos_sin, cos_rows, q_out, (uint32_t*)k_codes,
+               (uint32_t*)k_scales, (uint32_t*)v_codes, (uint32_t*)v_scales};
+  const int64_t blocks = (a.rows * (head_dim / 8) + 255) / 256;
+  if (blocks > 0x7FFFFFFF) return BF16X_ESHAPE;
+#define APPEND(D, T) \
+  hipLaunchKernelGGL((kv4_append_kernel<D, T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
+  if (head_dim == 128) {
+    if (type == BF16X_BF16) APPEND(128, BF16X_BF16);
+    else if (type == BF16X_F16) APPEND(128, BF16X_F16);
+    else APPEND(128, BF16X_F32);
+  } else {
+    if (type == BF16X_BF16) APPEND(64, BF16X_BF16);
+    else if (type == BF16X_F16) APPEND(64, BF16X_F16);
+    else APPEND(64, BF16X_F32);
+  }
+#undef APPEND
+  return launch_status();
+}
+
+extern "C" int bf16x_kv4_read(const uint8_t* k_codes, const uint16_t* k_scales, const uint8_t* v_codes,
+                              const uint16_t* v_scales, int64_t batch, int64_t tokens, int64_t n_kv_heads,
+                              int64_t head_dim, int64_t max_len, const int32_t* pos, int32_t type, void* k_out,
+                              void* v_out, bf16x_stream_t stream) {
+  if (!k_codes || !k_scales || !v_codes || !v_scales || !pos || !k_out || !v_out) return BF16X_EARG;
+  if (type != BF16X_BF16 && type != BF16X_F16 && type != BF16X_F32) return BF16X_EDTYPE;
+  const int bad = check_cache(batch, tokens, n_kv_heads, head_dim, max_len);
+  if (bad) return bad;
+  if (!aligned4(k_codes) || !aligned4(k_scales) || !aligned4(v_codes) || !aligned4(v_scales) || !aligned4(pos) ||
+      !aligned16(k_out) || !aligned16(v_out))
+    return BF16X_EARG;
+  if (batch == 0 || tokens == 0) return BF16X_OK;
+  ReadArgs a{(const uint32_t*)k_codes, (const uint32_t*)k_scales, (const uint32_t*)v_codes, (const uint32_t*)v_scales,
+             2 * batch * tokens * n_kv_heads, (int)tokens, (int)n_kv_heads, (int)max_len, pos, k_out, v_out};
+  const int64_t blocks = (a.rows * (head_dim / 8) + 255) / 256;
+  if (blocks > 0x7FFFFFFF) return BF16X_ESHAPE;
+#define READ(D, T) hipLaunchKernelGGL((kv4_read_kernel<D, T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
+  if (head_dim == 128) {
+    if (type == BF16X_BF16) READ(128, BF16X_BF16);
+    else if (type == BF16X_F16) READ(128, BF16X_F16);
+    else READ(128, BF16X_F32);
+  } else {
+    if (type == BF16X_BF16) READ(64, BF16X_BF16);
+    else if (type == BF16X_F16) READ(64, BF16X_F16);
+    else READ(64, BF16X_F32);
+  }
+#undef READ
+  return launch_status();
+}
+
+extern "C" int64_t bf16x_kv4_attention_workspace(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                                                 int64_t head_dim, int64_t max_len) {
+  if (check_cache(batch, tokens, n_kv_heads, head_dim, max_len) || n_heads <= 0 || n_heads % n_kv_heads) return -1;
+  const int64_t rows = tokens * (n_heads / n_kv_heads);
+  const Cut cut = cut_of(batch, rows, n_kv_heads, max_len);
+  return cut.splits == 1 ? 0 : cut.splits * batch * n_kv_heads * rows * (head_dim + 2) * 4;
+}
+
+extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int32_t type,
+                                   int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                                   int64_t head_dim, int64_t max_len, const uint8_t* k_codes,
+                                   const uint16_t* k_scales, const uint8_t* v_codes, const uint16_t* v_scales,
+                                   const int32_t* pos, const int32_t* start, int64_t window, float scale, void* out,
+                                   void* workspace, int64_t workspace_bytes, bf16x_stream_t stream) {
+  if (!q || !k_codes || !k_scales || !v_codes || !v_scales || !pos || !out || window < 0) return BF16X_EARG;
+  if (!is_half(type)) return BF16X_EDTYPE;
+  const int bad = check_cache(batch, tokens, n_kv_heads, head_dim, max_len);
+  if (bad) return bad;
+  if (n_heads <= 0 || n_heads > 65535 || n_heads % n_kv_heads) return BF16X_ESHAPE;
+  if (!rows_aligned(q, q_sb, q_st, q_sh, 2) || !aligned16(k_codes) || !aligned4(k_scales) || !aligned4(v_codes) ||
+      !aligned4(v_scales) || !aligned4(pos) || !aligned4(start) || !aligned4(out) || !aligned16(workspace))
+    return BF16X_EARG;
+  const int64_t need = bf16x_kv4_attention_workspace(batch, tokens, n_heads, n_kv_heads, head_dim, max_len);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return BF16X_ECAPACITY;
+  if (batch == 0 || tokens == 0) return BF16X_OK;
+  const int64_t G = n_heads / n_kv_heads, rows = tokens * G;
+  const Cut cut = cut_of(batch, rows, n_kv_heads, max_len);
+  const int64_t blocks = batch * n_kv_heads * cut.tiles * cut.splits;
+  if (rows > 0x3FFFFFFF || blocks > 0x7FFFFFFF || batch * n_kv_heads * rows > 0x7FFFFFFF) return BF16X_ESHAPE;
+  // a window of max_len + tokens keys or more bounds nothing
+  const int64_t win = std::min<int64_t>(window, 0x7FFFFFFF);
+  AttnArgs a{(const uint16_t*)q, q_sb, q_st, q_sh, (int)batch, (int)tokens, (int)n_heads, (int)n_kv_heads, (int)G,
+             (int)max_len, (int)rows, cut.tiles, cut.splits, (int)win, scale, k_codes, (const uint32_t*)k_scales,
+             v_codes, (const uint32_t*)v_scales, pos, start, (uint16_t*)out, (float*)workspace};
+  const hipStream_t st = (hipStream_t)stream;
+#define ROWS(D, BF) hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, st, a)
+#define JOIN(D, BF) \
+  hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)(batch * n_kv_heads * rows)), dim3(D), 0, st, a)
+  const bool bf = type == BF16X_BF16;
+  if (head_dim == 128) {
+    if (bf) ROWS(128, true);
+    else ROWS(128, false);
+  } else {
+    if (bf) ROWS(64, true);
+    else ROWS(64, false);
+  }
+  if (cut.splits > 1) {
+    if (head_dim == 128) {
+      if (bf) JOIN(128, true);
+      else JOIN(128, false);
+    } else {
+      if (bf) JOIN(64, true);
+      else JOIN(64, false);
+    }
+  }
+#undef ROWS
+#undef JOIN
+  return launch_status();
+}

@@ -1,0 +1,93 @@
+"""A KV cache held in 4 bits: append (with the rotary embedding), read back,
+attention.
+
+The reference's harness (bench_fused_cpm5.py:27-57) keeps a 16-bit cache inside
+Hugging Face modules; this cache takes 80 bytes per token and head instead of
+256 (head_dim 128), so the same memory holds 3.2 times the context, and a decode
+step reads that much less.  The format (codes, scales, rounding) is in
+include/bf16x_llama.h; the kernels are csrc/kv4.hip.
+
+    cache = kv4.Kv4Cache.zeros(batch, n_kv_heads, max_len, device="cuda")
+    q = kv4.append(k, v, cache, pos, q=q, cos_sin=table)      # rotates q and k, writes the rows
+    y = kv4.attention(q, cache, pos)                          # one token per sequence, or a prompt
+
+`cache` is a Kv4Cache or any tuple of its four tensors.  Positions are on the
+device, so a decode step can be captured in a HIP graph.  There is no backward
+pass: the cache is for generation.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+
+__all__ = ["Kv4Cache", "append", "read", "attention"]
+
+_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+
+
+class Kv4Cache(NamedTuple):
+    """k, v: uint8 [batch, n_kv_heads, max_len, head_dim / 2]; k_scale, v_scale:
+    fp16 [batch, n_kv_heads, max_len, head_dim / 32, 2], (scale, minimum) of
+    each group of 32 values.  Contiguous, on one GPU; head_dim 64 or 128."""
+    k: torch.Tensor
+    k_scale: torch.Tensor
+    v: torch.Tensor
+    v_scale: torch.Tensor
+
+    @classmethod
+    def zeros(cls, batch: int, n_kv_heads: int, max_len: int, head_dim: int = 128, device=None) -> "Kv4Cache":
+        if head_dim not in (64, 128):
+            raise ValueError("head_dim must be 64 or 128")
+        if min(n_kv_heads, max_len) < 1 or batch < 0:
+            raise ValueError("a cache needs at least one head and one row")
+        codes = lambda: torch.zeros(batch, n_kv_heads, max_len, head_dim // 2, dtype=torch.uint8, device=device)
+        scales = lambda: torch.zeros(batch, n_kv_heads, max_len, head_dim // 32, 2, dtype=torch.float16, device=device)
+        return cls(codes(), scales(), codes(), scales())
+
+    @property
+    def max_len(self) -> int:
+        return self.k.shape[2]
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self)
+
+
+def append(k, v, cache, pos, q=None, cos_sin=None):
+    """Write k, v [batch, tokens, n_kv_heads, head_dim] (bf16, fp16 or fp32, any
+    strides) as rows pos[b] + t of each sequence; pos int32 [batch].  Rows
+    outside the cache are dropped.
+
+    cos_sin (fp32 [positions, head_dim / 2, 2], as llama.rope_table): k is
+    rotated at its position first, and q [batch, tokens, n_heads, head_dim] too,
+    if given: the rotated q is returned (a new tensor)."""
+    r = _lib.host().kv4_append(k, v, cache, pos, q, cos_sin)
+    if isinstance(r, int):
+        _lib.check(r, "bf16x_kv4_append")
+    return r
+
+
+def read(cache, pos, tokens: int, dtype=torch.bfloat16):
+    """(k, v) [batch, tokens, n_kv_heads, head_dim]: the values of rows pos[b] ..
+    pos[b] + tokens - 1; zeros for rows outside the cache."""
+    if dtype not in _TYPES:
+        raise TypeError(f"dtype must be bf16, fp16 or fp32, not {dtype}")
+    r = _lib.host().kv4_read(cache, pos, tokens, _TYPES[dtype])
+    if isinstance(r, int):
+        _lib.check(r, "bf16x_kv4_read")
+    return r
+
+
+def attention(q, cache, pos, start=None, window: int = 0, scale=None, out=None):
+    """Attention of q [batch, tokens, n_heads, head_dim] (bf16 or fp16) over the
+    cache.  Query t of sequence b stands at position p = pos[b] + t and sees keys
+    start[b] <= j <= p (start int32 [batch], default 0: left padding) with
+    p - window < j where window is not 0 (sliding window).  A query that sees no
+    key gives zeros.  scale defaults to head_dim ** -0.5; out: a contiguous
+    tensor of q's shape and type."""
+    r = _lib.host().kv4_attention(q, cache, pos, start, window, scale, out)
+    if isinstance(r, int):
+        _lib.check(r, "bf16x_kv4_attention")
+    return r

@@ -1,6 +1,8 @@
 /*
  * bf16x_llama.h -- decoder-stack kernels of the Llama-style harness that
- * drives the BF16X linears (libbf16x_hip.so, same library as bf16x_hip.h).
+ * drives the BF16X linears, and the serving operators beside them: a KV cache
+ * held in 4 bits and token sampling (libbf16x_hip.so, same library as
+ * bf16x_hip.h).
  *
  * None of these entry points has a counterpart in the reference's own code:
  * the reference's harness (bench_fused_cpm5.py:27-57) runs the ops between the
@@ -199,6 +201,114 @@ int64_t bf16x_greedy_workspace_bytes(void);
  * overlap (stream order, one graph replay at a time). */
 int bf16x_greedy(const uint16_t* logits, int64_t vocab, int64_t* token, int32_t* state, int32_t* history,
                  int64_t history_len, void* workspace, int64_t workspace_bytes, bf16x_stream_t stream);
+
+/* Serving: a KV cache held in 4 bits with the attention that reads it, and
+ * token sampling.  (The reference's harness keeps a 16-bit cache inside Hugging
+ * Face modules and takes the most likely token.)
+ *
+ * The 4-bit cache
+ *  - codes   uint8 [batch][n_kv_heads][max_len][head_dim / 2]
+ *  - scales  fp16 [batch][n_kv_heads][max_len][head_dim / 32][2]: (scale,
+ *            minimum) of each group of 32 consecutive values of a row
+ *  A value is minimum + scale * code, code 0 .. 15.  A group is quantised as
+ *    minimum = fp16(min x), scale = fp16(max(0, max x - minimum) / 15),
+ *    code = round((x - minimum) / scale), half to even, cut to 0 .. 15 (0 where
+ *    the scale is 0), in fp32.
+ *  Values are cut to +-61440 first and a NaN counts as 0, so scales and minima
+ *  written here are always finite, and so is every value in fp16.
+ *  The codes of values 8w .. 8w + 7 of a row are its 4-byte word w, value
+ *  8w + 2i at bits 4i .. 4i + 3 and value 8w + 2i + 1 at bits 16 + 4i .. 19 +
+ *  4i, so that one mask takes the codes of two neighbouring values into the two
+ *  halves of a word.
+ *
+ * head_dim is 64 or 128.  Activations are bf16 or fp16 (BF16X_BF16 / _F16);
+ * append and read also take BF16X_F32.  Strides are in elements; the values of
+ * a head are contiguous, and heads start at multiples of 16 bytes.
+ */
+
+/* Appends `tokens` rows of K and V to each sequence's cache: token t of
+ * sequence b is row pos[b] + t; rows outside [0, max_len) are not written.
+ * With cos_sin (fp32 [cos_rows][head_dim / 2][2], (cos, sin) of a position,
+ * pairs (i, i + head_dim / 2)) K is rotated first, in fp32 and without a
+ * rounding before the quantisation, and q (n_heads heads; NULL: none), rotated
+ * the same way, is written to q_out [batch][tokens][n_heads][head_dim] in its
+ * own type.  Positions are cut to [0, cos_rows) for the table.  Without
+ * cos_sin q must be NULL. */
+int bf16x_kv4_append(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
+                     int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, int32_t type, int64_t batch,
+                     int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_len,
+                     const int32_t* pos, const float* cos_sin, int64_t cos_rows, void* q_out, uint8_t* k_codes,
+                     uint16_t* k_scales, uint8_t* v_codes, uint16_t* v_scales, bf16x_stream_t stream);
+
+/* The values of rows pos[b] .. pos[b] + tokens - 1 of each sequence, k_out and
+ * v_out [batch][tokens][n_kv_heads][head_dim] in `type`; zeros for rows outside
+ * [0, max_len). */
+int bf16x_kv4_read(const uint8_t* k_codes, const uint16_t* k_scales, const uint8_t* v_codes, const uint16_t* v_scales,
+                   int64_t batch, int64_t tokens, int64_t n_kv_heads, int64_t head_dim, int64_t max_len,
+                   const int32_t* pos, int32_t type, void* k_out, void* v_out, bf16x_stream_t stream);
+
+/* Grouped-query attention over the 4-bit cache: query t of sequence b stands at
+ * position p = pos[b] + t and sees the keys j with
+ *   start[b] <= j (start NULL: 0), p - window < j (window 0: no bound),
+ *   j <= p and j < max_len;
+ * out = softmax(scale q . K) V, zeros for a query that sees no key.  Query head
+ * h reads KV head h / (n_heads / n_kv_heads).  q [batch][tokens][n_heads]
+ * [head_dim] with its strides, out contiguous in the same order, both in `type`
+ * (bf16 or fp16).  Products are fp16 MFMA with fp32 sums: q is scaled by a power
+ * of two into fp16's range, the cached values and the softmax's weights are
+ * rounded to fp16 (11 bits); maxima, sums and the output are held in fp32.
+ * The keys of a query tile may be split over workgroups that leave partial
+ * results in `workspace` (bf16x_kv4_attention_workspace bytes, 16-byte aligned,
+ * any contents; may be NULL where that is 0). */
+int64_t bf16x_kv4_attention_workspace(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                                      int64_t head_dim, int64_t max_len);
+int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int32_t type, int64_t batch,
+                        int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_len,
+                        const uint8_t* k_codes, const uint16_t* k_scales, const uint8_t* v_codes,
+                        const uint16_t* v_scales, const int32_t* pos, const int32_t* start, int64_t window,
+                        float scale, void* out, void* workspace, int64_t workspace_bytes, bf16x_stream_t stream);
+
+/* Settings of bf16x_sample: one value for all rows, or with a pointer one per
+ * row, on the device. */
+typedef struct {
+  const float* temperature; /* NULL: temperature_all, and so on */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+} bf16x_sample_settings;
+
+/* Draws one token per row of logits [rows][vocab] (bf16, fp16 or fp32, rows
+ * row_stride elements apart) from the uniform numbers u[rows] in [0, 1).
+ * With m the row's largest logit, x_i its logits and T its temperature,
+ *   w_i = exp((x_i - m) / T);
+ *   top_k  keeps the first top_k tokens by (larger x, then lower index)
+ *          (<= 0 or >= vocab: all),
+ *   top_p  of those the shortest prefix whose weight is at least top_p of
+ *          theirs, never less than one token (>= 1: all),
+ *   min_p  of those the tokens with w_i >= min_p (cut to at most 1);
+ * the token is the first kept one, by index, at which the running sum of the
+ * kept weights passes u times their sum (u is cut to [0, 1)).  T = 0 (or
+ * anything not above 0) takes the first maximum.  A logit of -inf or NaN is
+ * never drawn; with a logit of +inf only the +inf tokens are.  A row without any
+ * other logit gives token -1.  Weights are computed in fp64 and summed as
+ * integers of 2^-44, so the result does not depend on an order of summation; a
+ * token below 2^-45 of the likeliest is not drawn.
+ * token int64 [rows]; logprob fp32 [rows] or NULL: the logarithm of the token's
+ * probability among the kept ones (0 for T = 0, -inf for token -1).
+ * state (NULL: none; rows must be 1): int32[2] {position, number of tokens in
+ * history}; u is then u[state[1]] of n_u numbers (the last where it is beyond),
+ * history[state[1]] = token when state[1] < history_len, and both counts go up
+ * by one.  vocab <= 1048576.  workspace: bf16x_sample_workspace bytes, 16-byte
+ * aligned, any contents. */
+int64_t bf16x_sample_workspace(int64_t rows, int64_t vocab);
+int bf16x_sample(const void* logits, int32_t type, int64_t row_stride, int64_t rows, int64_t vocab, const float* u,
+                 int64_t n_u, const bf16x_sample_settings* settings, int64_t* token, float* logprob, int32_t* state,
+                 int32_t* history, int64_t history_len, void* workspace, int64_t workspace_bytes,
+                 bf16x_stream_t stream);
 
 #ifdef __cplusplus
 }
