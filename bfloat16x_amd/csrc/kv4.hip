@@ -464,29 +464,305 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
   }
 }
 
-// Joins the splits of a row: one workgroup of D threads per row.
+// Many query rows (prompts): a tile of 128 rows, 32 per wave as two column
+// blocks of the MFMA; the cache goes through LDS in blocks of 64 keys, made
+// into fp16 once for all 128 rows, K as rows (padded by 16 bytes) and V
+// transposed (rows of 128 bytes, 16-byte columns exchanged by the row's word, so
+// that neither the writes nor the operand reads of 8 lanes meet in a bank).  Row
+// NT r + n of the transposed block holds nibble n of word r: MFMA row r of
+// product n.  Two buffers, one barrier per block; the next block's codes are in
+// registers while this one is multiplied.
+constexpr int kTileRows = 128;
+constexpr int kBlock = 64;                 // keys
+
+// Maximum over the 4 lanes that hold a row's keys (lanes c, c + 16, c + 32, c + 48).
+__device__ __forceinline__ float row_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 template <int D, bool BF>
-__global__ __launch_bounds__(D) void kv4_attn_join_kernel(AttnArgs a) {
-  const int64_t all = (int64_t)a.batch * a.KV * a.rows, at = blockIdx.x;
-  const int d = threadIdx.x;
-  const float* ml = a.part + a.splits * all * D;
-  float M = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[2 * (s * all + at)]);
-  const float from = M == -INFINITY ? 0.f : M;
-  float L = 0.f, y = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t i = s * all + at;
-    const float f = __builtin_amdgcn_exp2f(ml[2 * i] - from);
-    L = fmaf(ml[2 * i + 1], f, L);
-    y = fmaf(a.part[i * D + d], f, y);
+__global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
+  constexpr int W = D / 32, NT = D / 16, KW = D / 32;           // KW: words of codes a thread stages of a key
+  constexpr int KROW = 2 * D + 16, VROW = 2 * kBlock;
+  __shared__ __attribute__((aligned(16))) uint8_t kls[2][kBlock * KROW];
+  __shared__ __attribute__((aligned(16))) uint8_t vls[2][D * VROW];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // heads fastest, so that a head's tiles share an XCD's L2 where there are 8; the last tiles, which see the most
+  // keys, first
+  int id = blockIdx.x;
+  const int kvh = id % a.KV;
+  id /= a.KV;
+  const int b = id % a.batch;
+  id /= a.batch;
+  const int sp = id % a.splits, tile = a.tiles - 1 - id / a.splits;
+  const int r0 = kTileRows * tile, w0 = r0 + 32 * w;
+  int lo[2], hi[2], LO, HI, wlo = 0, whi = 0, flo = 0, fhi = 0, unused;
+  key_range(a, b, r0 / a.G, LO, unused);
+  key_range(a, b, min(r0 + kTileRows - 1, a.rows - 1) / a.G, unused, HI);
+  if (w0 < a.rows) {                       // keys some row of the wave sees, and keys all of them see
+    key_range(a, b, w0 / a.G, wlo, fhi);
+    key_range(a, b, min(w0 + 31, a.rows - 1) / a.G, flo, whi);
   }
+  const int base = LO & ~(kBlock - 1);
+  const int blocks = HI > LO ? (HI - base + kBlock - 1) / kBlock : 0;
+  const int per = (blocks + a.splits - 1) / a.splits;
+  const int b0 = sp * per, b1 = min(b0 + per, blocks);
+
+  const int64_t head = ((int64_t)b * a.KV + kvh) * a.max_len;
+  const uint8_t *kc = a.kc + head * (D / 2), *vc = a.vc + head * (D / 2);
+  const uint32_t *ks = a.ks + head * (D / 32), *vs = a.vs + head * (D / 32);
+
+  // staging: thread (key, quarter of its codes) of K, (word, 4 keys) of V, the upper half of the word's nibbles being
+  // another thread's where D is 64
+  const int kkey = tid >> 2, kpart = tid & 3;
+  const int vw = tid & (D / 8 - 1), vhalf = D == 64 ? (tid >> 3) & 1 : 0, vr = vw + 8 * vhalf, vquad = tid >> 4;
+  uint32_t kr[KW], ksr, vr_[4], vsr[4];
+  auto load_block = [&](int blk) {
+    const int j0 = base + kBlock * blk, last = a.max_len - 1;
+    const int64_t j = min(j0 + kkey, last);
+    if constexpr (D == 128) {
+      const u32x4 x = *(const u32x4*)(kc + j * (D / 2) + 16 * kpart);
+      kr[0] = x.x, kr[1] = x.y, kr[2] = x.z, kr[3] = x.w;
+      ksr = ks[j * (D / 32) + kpart];
+    } else {
+      const uint2 x = *(const uint2*)(kc + j * (D / 2) + 8 * kpart);
+      kr[0] = x.x, kr[1] = x.y;
+      ksr = ks[j * (D / 32) + (kpart >> 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int jv = j0 + 4 * vquad + e;
+      const int64_t jc = min(jv, last);
+      vr_[e] = *(const uint32_t*)(vc + jc * (D / 2) + 4 * vw);
+      vsr[e] = jv >= LO && jv < HI ? vs[jc * (D / 32) + vw / 4] : 0u;       // keys that no row sees have value 0
+    }
+  };
+  auto store_block = [&](int slot) {
+    uint8_t* kd = kls[slot] + kkey * KROW + kpart * (D / 2);
+    const h2 s = scale_of(ksr), m = minimum_of(ksr);
+#pragma unroll
+    for (int i = 0; i < KW; ++i) *(h8*)(kd + 16 * i) = word_values(kr[i], s, m);
+    const int col = 4 * (vquad >> 3) + (vquad & 3);
+    uint8_t* vd = vls[slot] + NT * vr * VROW + ((col ^ (vr & 7)) * 16) + ((vquad >> 2) & 1) * 8;
+    uint32_t two[2][NT];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const h2 s2 = as_h2(__builtin_amdgcn_perm(vsr[2 * k + 1], vsr[2 * k], 0x05040100u));
+      const h2 m2 = as_h2(__builtin_amdgcn_perm(vsr[2 * k + 1], vsr[2 * k], 0x07060302u));
+      uint32_t va = vr_[2 * k], vb = vr_[2 * k + 1];
+      if constexpr (D == 64) {
+        va = vhalf ? va >> 16 : va;
+        vb = vhalf ? vb >> 16 : vb;
+      }
+#pragma unroll
+      for (int y = 0; y < NT / 2; ++y) {
+        const uint32_t x = __builtin_amdgcn_perm(vb, va, 0x0C040C00u + 0x00010001u * y);
+        two[k][2 * y] = as_u32(__builtin_elementwise_fma(low_codes(x), s2, m2));
+        two[k][2 * y + 1] = as_u32(__builtin_elementwise_fma(high_codes(x), s2, m2));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *(uint2*)(vd + n * VROW) = make_uint2(two[0][n], two[1][n]);
+  };
+
+  if (b0 < b1) load_block(b0);
+  h8 qb[2][W];
+  float sc[2];
+  int qoff[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) qoff[i] = 32 * i + 8 * g;
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    const int r = w0 + 16 * ct + c, rc = min(r, a.rows - 1), t = rc / a.G, hg = rc - t * a.G;
+    key_range(a, b, t, lo[ct], hi[ct]);
+    sc[ct] = a.scale * kLog2e *
+             load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, r < a.rows, qb[ct], qoff);
+  }
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  f4 o[2][NT];
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[ct][n] = f4{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](int blk, int slot) {
+    const int j0 = base + kBlock * blk;
+    if (j0 >= whi || j0 + kBlock <= wlo) return;                // (the wave as a whole)
+    f4 s[2][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      s[0][kt] = s[1][kt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const h8 kk = *(const h8*)(kls[slot] + (16 * kt + c) * KROW + 64 * i + 16 * g);
+        s[0][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qb[0][i], s[0][kt], 0, 0, 0);
+        s[1][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qb[1][i], s[1][kt], 0, 0, 0);
+      }
+    }
+    const bool whole = j0 >= flo && j0 + kBlock <= fhi;
+    h8 p[2][2];
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+      float mb = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float x = s[ct][kt][v] * sc[ct];
+          if (!whole) {
+            const int j = j0 + 16 * kt + 4 * g + v;
+            x = j >= lo[ct] && j < hi[ct] ? x : -INFINITY;
+          }
+          s[ct][kt][v] = x;
+          mb = fmaxf(mb, x);
+        }
+      mb = row_max(mb);
+      // weights may grow to 2^8 of the maximum that they are taken against before it is renewed: the sums are fp32 and
+      // 2^8 is well inside fp16, and most blocks leave the outputs unscaled
+      if (__any(mb > m[ct] + 8.f)) {
+        const float mn = fmaxf(m[ct], mb);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mn);
+        m[ct] = mn;
+        l[ct] *= alpha;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[ct][n] *= alpha;
+      }
+      const float from = m[ct] == -INFINITY ? 0.f : m[ct];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float e = __builtin_amdgcn_exp2f(s[ct][kt][v] - from);
+          l[ct] += e;
+          p[ct][kt >> 1][4 * (kt & 1) + v] = (_Float16)e;
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const h8 vv = *(const h8*)(vls[slot] + (NT * c + n) * VROW + (((4 * h + g) ^ (c & 7)) * 16));
+        o[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[0][h], o[0][n], 0, 0, 0);
+        o[1][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[1][h], o[1][n], 0, 0, 0);
+      }
+  };
+
+  if (b0 < b1) {
+    store_block(0);
+    if (b0 + 1 < b1) load_block(b0 + 1);
+  }
+  __syncthreads();
+  for (int blk = b0; blk < b1; ++blk) {
+    const int slot = (blk - b0) & 1;
+    if (blk + 1 < b1) {                    // into the other buffer, whose readers passed the last barrier
+      store_block(slot ^ 1);
+      if (blk + 2 < b1) load_block(blk + 2);
+    }
+    compute(blk, slot);
+    __syncthreads();
+  }
+
+  const int64_t all = (int64_t)a.batch * a.KV * a.rows;
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    float L = l[ct];
+    L += __shfl_xor(L, 16, 64);
+    L += __shfl_xor(L, 32, 64);
+    const int r = w0 + 16 * ct + c;
+    if (r >= a.rows) continue;
+    const int t = r / a.G, hg = r - t * a.G;
+    const int64_t at = sp * all + ((int64_t)b * a.KV + kvh) * a.rows + r;
+    if (a.splits > 1 && g == 0) {
+      float* ml = a.part + a.splits * all * D + 2 * at;
+      ml[0] = m[ct];
+      ml[1] = L;
+    }
+    const float inv = a.splits > 1 ? 1.f : L > 0.f ? 1.f / L : 0.f;
+    uint16_t* op = a.out + (((int64_t)b * a.tokens + t) * a.H + kvh * a.G + hg) * D;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int rr = 4 * g + v;
+      float y[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) y[n] = o[ct][n][v] * inv;
+      if constexpr (D == 128) {            // nibbles 0 .. 7 are values 0, 2, 4, 6, 1, 3, 5, 7 of the word
+        if (a.splits > 1) {
+          float* pp = a.part + at * D + 8 * rr;
+          *(f4*)pp = f4{y[0], y[4], y[1], y[5]};
+          *(f4*)(pp + 4) = f4{y[2], y[6], y[3], y[7]};
+        } else {
+          *(u32x4*)(op + 8 * rr) = u32x4{out2<BF>(y[0], y[4]), out2<BF>(y[1], y[5]), out2<BF>(y[2], y[6]),
+                                         out2<BF>(y[3], y[7])};
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int d = 8 * (rr & 7) + 2 * n + (rr >> 3);
+          if (a.splits > 1) a.part[at * D + d] = y[n];
+          else op[d] = (uint16_t)out2<BF>(y[n], 0.f);
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one workgroup per row, D / 4 lanes per split, so
+// that all partial results of the row are requested at once.
+constexpr int kMaxSplits = 128;
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a) {
+  constexpr int LS = D / 4, NG = 256 / LS, E = kMaxSplits / NG;
+  __shared__ f4 sum[NG][LS];
+  const int64_t all = (int64_t)a.batch * a.KV * a.rows, at = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, grp = tid / LS, d = tid % LS;
+  const float* ml = a.part + a.splits * all * D;
+  float mv[kMaxSplits / 64], lv[kMaxSplits / 64], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMaxSplits / 64; ++k) {
+    const int s = lane + 64 * k;
+    mv[k] = s < a.splits ? ml[2 * (s * all + at)] : -INFINITY;
+    lv[k] = s < a.splits ? ml[2 * (s * all + at) + 1] : 0.f;
+    M = fmaxf(M, mv[k]);
+  }
+  f4 v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int s = grp + NG * e;
+    v[e] = s < a.splits ? *(const f4*)(a.part + (s * all + at) * D + 4 * d) : f4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float from = M == -INFINITY ? 0.f : M;
+  float f[kMaxSplits / 64];
+#pragma unroll
+  for (int k = 0; k < kMaxSplits / 64; ++k) {
+    f[k] = __builtin_amdgcn_exp2f(mv[k] - from);
+    L = fmaf(lv[k], f[k], L);
+  }
+  L = wave_sum(L);
+  f4 y = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int s = grp + NG * e;
+    y += v[e] * __shfl(f[NG * e / 64], s & 63, 64);
+  }
+  sum[grp][d] = y;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int k = 1; k < NG; ++k) y += sum[k][d];
   const int64_t bk = at / a.rows;
   const int r = (int)(at - bk * a.rows), t = r / a.G, hg = r - t * a.G;
   const int64_t b = bk / a.KV;
   const int kvh = (int)(bk - b * a.KV);
-  const float v = y * (L > 0.f ? 1.f / L : 0.f);
-  a.out[((b * a.tokens + t) * a.H + kvh * a.G + hg) * D + d] =
-      BF ? (uint16_t)f32_to_bf16_rne(v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+  y *= L > 0.f ? 1.f / L : 0.f;
+  *(uint2*)(a.out + ((b * a.tokens + t) * a.H + kvh * a.G + hg) * D + 4 * d) =
+      make_uint2(out2<BF>(y[0], y[1]), out2<BF>(y[2], y[3]));
 }
 
 // ---------------------------------------------------------------------------
@@ -508,15 +784,18 @@ bool rows_aligned(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t siz
   return aligned16(p) && sb * size % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
 }
 
-// How the work of an attention call is cut: tiles of 16 query rows, and splits
-// of their keys so that a small call still fills the card.
+// How the work of an attention call is cut: tiles of 16 query rows (few rows)
+// or of 128, and splits of their keys so that a small call still fills the card.
 struct Cut {
+  bool wide;
   int tiles, splits;
 };
 Cut cut_of(int64_t batch, int64_t rows, int64_t KV, int64_t max_len) {
-  const int64_t tiles = (rows + 15) / 16, wgs = batch * KV * tiles;
-  const int64_t want = wgs > 0 ? 512 / wgs : 1, most = (max_len + 32 * kRowWaves - 1) / (32 * kRowWaves);
-  return {(int)tiles, (int)std::max<int64_t>(1, std::min<int64_t>({want, most, 128}))};
+  const bool wide = rows > 64;
+  const int64_t tile = wide ? kTileRows : 16, keys = wide ? 512 : 32 * kRowWaves;
+  const int64_t tiles = (rows + tile - 1) / tile, wgs = batch * KV * tiles;
+  const int64_t want = wgs > 0 ? 512 / wgs : 1, most = (max_len + keys - 1) / keys;
+  return {wide, (int)tiles, (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}))};
 }
 
 }  // namespace
@@ -610,7 +889,7 @@ extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, in
   if (bad) return bad;
   if (n_heads <= 0 || n_heads > 65535 || n_heads % n_kv_heads) return BF16X_ESHAPE;
   if (!rows_aligned(q, q_sb, q_st, q_sh, 2) || !aligned16(k_codes) || !aligned4(k_scales) || !aligned4(v_codes) ||
-      !aligned4(v_scales) || !aligned4(pos) || !aligned4(start) || !aligned4(out) || !aligned16(workspace))
+      !aligned4(v_scales) || !aligned4(pos) || !aligned4(start) || !aligned16(out) || !aligned16(workspace))
     return BF16X_EARG;
   const int64_t need = bf16x_kv4_attention_workspace(batch, tokens, n_heads, n_kv_heads, head_dim, max_len);
   if (need > 0 && (!workspace || workspace_bytes < need)) return BF16X_ECAPACITY;
@@ -626,10 +905,19 @@ extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, in
              v_codes, (const uint32_t*)v_scales, pos, start, (uint16_t*)out, (float*)workspace};
   const hipStream_t st = (hipStream_t)stream;
 #define ROWS(D, BF) hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, st, a)
+#define TILES(D, BF) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, BF>), dim3((unsigned)blocks), dim3(256), 0, st, a)
 #define JOIN(D, BF) \
-  hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)(batch * n_kv_heads * rows)), dim3(D), 0, st, a)
+  hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)(batch * n_kv_heads * rows)), dim3(256), 0, st, a)
   const bool bf = type == BF16X_BF16;
-  if (head_dim == 128) {
+  if (cut.wide) {
+    if (head_dim == 128) {
+      if (bf) TILES(128, true);
+      else TILES(128, false);
+    } else {
+      if (bf) TILES(64, true);
+      else TILES(64, false);
+    }
+  } else if (head_dim == 128) {
     if (bf) ROWS(128, true);
     else ROWS(128, false);
   } else {
@@ -646,6 +934,7 @@ extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, in
     }
   }
 #undef ROWS
+#undef TILES
 #undef JOIN
   return launch_status();
 }
