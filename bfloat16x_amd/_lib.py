@@ -129,6 +129,7 @@ TUNE_KEYS = {
     "gemm_ws_split": 5, "skinny_waves": 6, "skinny2_kq": 7, "skinny2_split": 8, "gemv_iters": 9, "gemv_g": 10,
     "gemv_long": 11, "gemv_xm_slots": 12, "gguf_long": 13, "gguf_iters": 14, "attn_split": 15,
     "gemm_ws_grouped": 16, "gemm_ws_resident": 17, "attn_mfma": 18, "chunk_atoms": 19, "gemm_ws_bm": 20, "gemm_stream_max": 21,
+    "kv4_tile": 22, "kv4_split": 23,
 }
 
 _LIB = None

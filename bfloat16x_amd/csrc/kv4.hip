@@ -33,15 +33,25 @@ constexpr float kLog2e = 1.44269504088896341f;
 __device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
 __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 
-// Codes of the low nibbles of bytes 0 and 2, or of their high nibbles.
-__device__ __forceinline__ h2 low_codes(uint32_t w) { return as_h2((w & 0x000F000Fu) | 0x64006400u) - h2{1024, 1024}; }
-__device__ __forceinline__ h2 high_codes(uint32_t w) { return as_h2((w & 0x00F000F0u) | 0x54005400u) - h2{64, 64}; }
+// Codes of the low nibbles of bytes 0 and 2, or of their high nibbles.  The
+// exponents are kept in a register that the compiler cannot see through: with
+// two literals it would take v_and_b32 and v_or_b32 instead of v_and_or_b32.
+struct Exponents {
+  uint32_t low = 0x64006400u, high = 0x54005400u;
+  __device__ __forceinline__ Exponents() { asm("" : "+v"(low), "+v"(high)); }
+};
+__device__ __forceinline__ h2 low_codes(uint32_t w, const Exponents& x) {
+  return as_h2((w & 0x000F000Fu) | x.low) - h2{1024, 1024};
+}
+__device__ __forceinline__ h2 high_codes(uint32_t w, const Exponents& x) {
+  return as_h2((w & 0x00F000F0u) | x.high) - h2{64, 64};
+}
 
 // The 8 values of a word of codes, in order; s = (scale, scale), m = (minimum, minimum).
-__device__ __forceinline__ h8 word_values(uint32_t w, h2 s, h2 m) {
-  const h2 a = __builtin_elementwise_fma(low_codes(w), s, m), b = __builtin_elementwise_fma(high_codes(w), s, m);
+__device__ __forceinline__ h8 word_values(uint32_t w, h2 s, h2 m, const Exponents& x) {
+  const h2 a = __builtin_elementwise_fma(low_codes(w, x), s, m), b = __builtin_elementwise_fma(high_codes(w, x), s, m);
   w >>= 8;
-  const h2 c = __builtin_elementwise_fma(low_codes(w), s, m), d = __builtin_elementwise_fma(high_codes(w), s, m);
+  const h2 c = __builtin_elementwise_fma(low_codes(w, x), s, m), d = __builtin_elementwise_fma(high_codes(w, x), s, m);
   return __builtin_bit_cast(h8, u32x4{as_u32(a), as_u32(b), as_u32(c), as_u32(d)});
 }
 // (scale, scale) and (minimum, minimum) of a scale word.
@@ -239,10 +249,12 @@ __device__ __forceinline__ uint32_t out2(float a, float b) {
 
 // The query operand of a lane: NW words of 2 values at `src` brought to fp16
 // by the power of two that puts the row's largest value (over the 4 lanes of
-// the row) into [1, 2); returns its inverse.  Exact for every value within
-// 2^-14 of the row's largest.
+// the row) into [1, 2), with the sign of `scale`; returns what a product's sum
+// is to be multiplied with for a score in powers of two, a positive number.
+// Exact for every value within 2^-14 of the row's largest.
 template <bool BF, int N>
-__device__ __forceinline__ float load_query(const uint16_t* src, bool valid, h8 (&qb)[N], const int (&off)[N]) {
+__device__ __forceinline__ float load_query(const uint16_t* src, bool valid, float scale, h8 (&qb)[N],
+                                            const int (&off)[N]) {
   float x[N][8];
   float mx = 0.f;
 #pragma unroll
@@ -257,12 +269,12 @@ __device__ __forceinline__ float load_query(const uint16_t* src, bool valid, h8 
   mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
   int e2 = (int)(__float_as_uint(mx) >> 23) - 127;
   e2 = mx > 0.f && e2 < 128 ? max(e2, -100) : 0;
-  const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+  const float down = copysignf(__uint_as_float((uint32_t)(127 - e2) << 23), scale);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) qb[i][e] = (_Float16)(x[i][e] * down);
-  return __uint_as_float((uint32_t)(127 + e2) << 23);
+  return fmaxf(fabsf(scale) * kLog2e * __uint_as_float((uint32_t)(127 + e2) << 23), 1.2e-38f);
 }
 
 // Few query rows (single tokens, drafts): a tile of 16 rows; 4 waves take the
@@ -335,14 +347,15 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
   int qoff[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) qoff[i] = g * (D / 4) + 8 * i;
-  const float back = load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, valid, qb, qoff);
-  const float sc = a.scale * kLog2e * back;
+  const float sc =
+      load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, valid, a.scale, qb, qoff);
 
   float m = -INFINITY, l = 0.f;
   f4 o[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
 
+  const Exponents ex;
   Step<D> cur, next;
   int s = sp * per + w;
   if (s < s1) load_step<D>(cur, kc, ks, vc, vs, base + 32 * s, a.max_len - 1, c, g);
@@ -358,7 +371,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
       f4 acc = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < W; ++i)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_values(cur.kc[kt][i], sc2, mn2), qb[i], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_values(cur.kc[kt][i], sc2, mn2, ex), qb[i], acc, 0, 0, 0);
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int j = j0 + 16 * kt + 4 * g + v;
@@ -401,8 +414,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
 #pragma unroll
       for (int y = 0; y < NT / 2; ++y) {
         const uint32_t two = __builtin_amdgcn_perm(vb, va, 0x0C040C00u + 0x00010001u * y);
-        av[2 * y][k] = as_u32(__builtin_elementwise_fma(low_codes(two), s2, m2));
-        av[2 * y + 1][k] = as_u32(__builtin_elementwise_fma(high_codes(two), s2, m2));
+        av[2 * y][k] = as_u32(__builtin_elementwise_fma(low_codes(two, ex), s2, m2));
+        av[2 * y + 1][k] = as_u32(__builtin_elementwise_fma(high_codes(two, ex), s2, m2));
       }
     }
 #pragma unroll
@@ -464,15 +477,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
   }
 }
 
-// Many query rows (prompts): a tile of 128 rows, 32 per wave as two column
+// Many query rows (prompts): a tile of 64 CT rows, 16 CT per wave as CT column
 // blocks of the MFMA; the cache goes through LDS in blocks of 64 keys, made
-// into fp16 once for all 128 rows, K as rows (padded by 16 bytes) and V
+// into fp16 once for all rows, K as rows (padded by 16 bytes) and V
 // transposed (rows of 128 bytes, 16-byte columns exchanged by the row's word, so
 // that neither the writes nor the operand reads of 8 lanes meet in a bank).  Row
 // NT r + n of the transposed block holds nibble n of word r: MFMA row r of
 // product n.  Two buffers, one barrier per block; the next block's codes are in
 // registers while this one is multiplied.
-constexpr int kTileRows = 128;
 constexpr int kBlock = 64;                 // keys
 
 // Maximum over the 4 lanes that hold a row's keys (lanes c, c + 16, c + 32, c + 48).
@@ -483,8 +495,9 @@ __device__ __forceinline__ float row_max(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <int D, bool BF>
+template <int D, int CT, bool BF>
 __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
+  constexpr int kTileRows = 64 * CT;
   constexpr int W = D / 32, NT = D / 16, KW = D / 32;           // KW: words of codes a thread stages of a key
   constexpr int KROW = 2 * D + 16, VROW = 2 * kBlock;
   __shared__ __attribute__((aligned(16))) uint8_t kls[2][kBlock * KROW];
@@ -499,13 +512,13 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   const int b = id % a.batch;
   id /= a.batch;
   const int sp = id % a.splits, tile = a.tiles - 1 - id / a.splits;
-  const int r0 = kTileRows * tile, w0 = r0 + 32 * w;
-  int lo[2], hi[2], LO, HI, wlo = 0, whi = 0, flo = 0, fhi = 0, unused;
+  const int r0 = kTileRows * tile, w0 = r0 + 16 * CT * w;
+  int lo[CT], hi[CT], LO, HI, flo = 0, fhi = 0, unused;
   key_range(a, b, r0 / a.G, LO, unused);
   key_range(a, b, min(r0 + kTileRows - 1, a.rows - 1) / a.G, unused, HI);
-  if (w0 < a.rows) {                       // keys some row of the wave sees, and keys all of them see
-    key_range(a, b, w0 / a.G, wlo, fhi);
-    key_range(a, b, min(w0 + 31, a.rows - 1) / a.G, flo, whi);
+  if (w0 < a.rows) {                       // keys that every row of the wave sees
+    key_range(a, b, w0 / a.G, unused, fhi);
+    key_range(a, b, min(w0 + 16 * CT - 1, a.rows - 1) / a.G, flo, unused);
   }
   const int base = LO & ~(kBlock - 1);
   const int blocks = HI > LO ? (HI - base + kBlock - 1) / kBlock : 0;
@@ -518,34 +531,54 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
 
   // staging: thread (key, quarter of its codes) of K, (word, 4 keys) of V, the upper half of the word's nibbles being
   // another thread's where D is 64
+  const Exponents ex;
   const int kkey = tid >> 2, kpart = tid & 3;
   const int vw = tid & (D / 8 - 1), vhalf = D == 64 ? (tid >> 3) & 1 : 0, vr = vw + 8 * vhalf, vquad = tid >> 4;
   uint32_t kr[KW], ksr, vr_[4], vsr[4];
-  auto load_block = [&](int blk) {
-    const int j0 = base + kBlock * blk, last = a.max_len - 1;
-    const int64_t j = min(j0 + kkey, last);
+  // (rows past the cache's end are its last one: the blocks' bases are uniform, offsets inside a block 32 bits)
+  auto load_k = [&](int blk) {
+    const int j0 = min(base + kBlock * blk, a.max_len - 1);
+    const uint32_t j = min(kkey, a.max_len - 1 - j0);
+    const uint8_t* kb = kc + (int64_t)j0 * (D / 2);
+    const uint32_t* sb = ks + (int64_t)j0 * (D / 32);
     if constexpr (D == 128) {
-      const u32x4 x = *(const u32x4*)(kc + j * (D / 2) + 16 * kpart);
+      const u32x4 x = *(const u32x4*)(kb + (j * (D / 2) + 16 * kpart));
       kr[0] = x.x, kr[1] = x.y, kr[2] = x.z, kr[3] = x.w;
-      ksr = ks[j * (D / 32) + kpart];
+      ksr = sb[j * (D / 32) + kpart];
     } else {
-      const uint2 x = *(const uint2*)(kc + j * (D / 2) + 8 * kpart);
+      const uint2 x = *(const uint2*)(kb + (j * (D / 2) + 8 * kpart));
       kr[0] = x.x, kr[1] = x.y;
-      ksr = ks[j * (D / 32) + (kpart >> 1)];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int jv = j0 + 4 * vquad + e;
-      const int64_t jc = min(jv, last);
-      vr_[e] = *(const uint32_t*)(vc + jc * (D / 2) + 4 * vw);
-      vsr[e] = jv >= LO && jv < HI ? vs[jc * (D / 32) + vw / 4] : 0u;       // keys that no row sees have value 0
+      ksr = sb[j * (D / 32) + (kpart >> 1)];
     }
   };
-  auto store_block = [&](int slot) {
+  auto load_v = [&](int blk) {
+    const int j0 = min(base + kBlock * blk, a.max_len - 1), last = a.max_len - 1 - j0;
+    const uint8_t* vb = vc + (int64_t)j0 * (D / 2);
+    const uint32_t* sb = vs + (int64_t)j0 * (D / 32);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t j = min(4 * vquad + e, last);
+      vr_[e] = *(const uint32_t*)(vb + (j * (D / 2) + 4 * vw));
+      vsr[e] = sb[j * (D / 32) + vw / 4];
+    }
+  };
+  auto store_k = [&](int slot) {
     uint8_t* kd = kls[slot] + kkey * KROW + kpart * (D / 2);
     const h2 s = scale_of(ksr), m = minimum_of(ksr);
 #pragma unroll
-    for (int i = 0; i < KW; ++i) *(h8*)(kd + 16 * i) = word_values(kr[i], s, m);
+    for (int i = 0; i < KW; ++i) *(h8*)(kd + 16 * i) = word_values(kr[i], s, m, ex);
+  };
+  // keys that no row sees have value 0, whatever their scales hold
+  auto hide_v = [&](int blk) {
+    const int j0 = base + kBlock * blk;
+    if (j0 >= LO && j0 + kBlock <= HI) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = j0 + 4 * vquad + e;
+      vsr[e] = ((j >= LO) & (j < HI)) ? vsr[e] : 0u;
+    }
+  };
+  auto store_v = [&](int slot) {
     const int col = 4 * (vquad >> 3) + (vquad & 3);
     uint8_t* vd = vls[slot] + NT * vr * VROW + ((col ^ (vr & 7)) * 16) + ((vquad >> 2) & 1) * 8;
     uint32_t two[2][NT];
@@ -561,124 +594,152 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
 #pragma unroll
       for (int y = 0; y < NT / 2; ++y) {
         const uint32_t x = __builtin_amdgcn_perm(vb, va, 0x0C040C00u + 0x00010001u * y);
-        two[k][2 * y] = as_u32(__builtin_elementwise_fma(low_codes(x), s2, m2));
-        two[k][2 * y + 1] = as_u32(__builtin_elementwise_fma(high_codes(x), s2, m2));
+        two[k][2 * y] = as_u32(__builtin_elementwise_fma(low_codes(x, ex), s2, m2));
+        two[k][2 * y + 1] = as_u32(__builtin_elementwise_fma(high_codes(x, ex), s2, m2));
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) *(uint2*)(vd + n * VROW) = make_uint2(two[0][n], two[1][n]);
   };
 
-  if (b0 < b1) load_block(b0);
-  h8 qb[2][W];
-  float sc[2];
+  if (b0 < b1) {
+    load_k(b0);
+    load_v(b0);
+  }
+  h8 qb[CT][W];
+  float sc[CT];
   int qoff[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) qoff[i] = 32 * i + 8 * g;
 #pragma unroll
-  for (int ct = 0; ct < 2; ++ct) {
+  for (int ct = 0; ct < CT; ++ct) {
     const int r = w0 + 16 * ct + c, rc = min(r, a.rows - 1), t = rc / a.G, hg = rc - t * a.G;
     key_range(a, b, t, lo[ct], hi[ct]);
-    sc[ct] = a.scale * kLog2e *
-             load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, r < a.rows, qb[ct], qoff);
+    sc[ct] = load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, r < a.rows, a.scale, qb[ct],
+                            qoff);
   }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  f4 o[2][NT];
+  // m: the maximum that the weights are taken against, in units of the products; l: their sums, from the same
+  // rounded weights as the outputs (a product with ones: all four registers hold the row's sum)
+  float m[CT];
+  f4 o[CT][NT], l[CT];
+  const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
-  for (int ct = 0; ct < 2; ++ct)
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY;
+    l[ct] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[ct][n] = f4{0.f, 0.f, 0.f, 0.f};
+  }
 
-  auto compute = [&](int blk, int slot) {
-    const int j0 = base + kBlock * blk;
-    if (j0 >= whi || j0 + kBlock <= wlo) return;                // (the wave as a whole)
-    f4 s[2][4];
+  // The products with K of block blk + 1 run beside the exponentials of block blk, and those with V of blk beside the
+  // staging of K of blk + 2 and V of blk + 1: matrix and vector pipes are both busy inside one wave.  (Blocks past
+  // the end are loaded from inside the cache and multiplied, and nothing of them is used.)
+  auto scores = [&](int slot, f4 (&s)[CT][4]) {
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      s[0][kt] = s[1][kt] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct][kt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const h8 kk = *(const h8*)(kls[slot] + (16 * kt + c) * KROW + 64 * i + 16 * g);
-        s[0][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qb[0][i], s[0][kt], 0, 0, 0);
-        s[1][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qb[1][i], s[1][kt], 0, 0, 0);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qb[ct][i], s[ct][kt], 0, 0, 0);
       }
     }
-    const bool whole = j0 >= flo && j0 + kBlock <= fhi;
-    h8 p[2][2];
+  };
+  f4 s[CT][4];
+  if (b0 < b1) {
+    store_k(0);
+    load_k(b0 + 1);
+    hide_v(b0);
+    store_v(0);
+    load_v(b0 + 1);
+    store_k(1);
+    load_k(b0 + 2);
+    __syncthreads();
+    scores(0, s);
+    __syncthreads();                       // (the loop's first staging overwrites that block of K)
+  }
+  for (int blk = b0; blk < b1; ++blk) {
+    const int slot = (blk - b0) & 1, j0 = base + kBlock * blk;
+    if (!(j0 >= flo && j0 + kBlock <= fhi)) {
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) {
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int j = j0 + 16 * kt + 4 * g + v;
+            s[ct][kt][v] = ((j >= lo[ct]) & (j < hi[ct])) ? s[ct][kt][v] : -INFINITY;
+          }
+    }
+    float from[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
       float mb = -INFINITY;
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          float x = s[ct][kt][v] * sc[ct];
-          if (!whole) {
-            const int j = j0 + 16 * kt + 4 * g + v;
-            x = j >= lo[ct] && j < hi[ct] ? x : -INFINITY;
-          }
-          s[ct][kt][v] = x;
-          mb = fmaxf(mb, x);
-        }
+        for (int v = 0; v < 4; ++v) mb = fmaxf(mb, s[ct][kt][v]);
       mb = row_max(mb);
       // weights may grow to 2^8 of the maximum that they are taken against before it is renewed: the sums are fp32 and
       // 2^8 is well inside fp16, and most blocks leave the outputs unscaled
-      if (__any(mb > m[ct] + 8.f)) {
+      if (__any((mb - m[ct]) * sc[ct] > 8.f)) {
         const float mn = fmaxf(m[ct], mb);
-        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[ct] - mn);
+        const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[ct] - mn) * sc[ct]);
         m[ct] = mn;
         l[ct] *= alpha;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[ct][n] *= alpha;
       }
-      const float from = m[ct] == -INFINITY ? 0.f : m[ct];
+      from[ct] = m[ct] == -INFINITY ? 0.f : -m[ct] * sc[ct];
+    }
+    hide_v(blk + 1);
+    h8 p[CT][2];
+    f4 next[CT][4];
+    scores(slot ^ 1, next);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float e = __builtin_amdgcn_exp2f(s[ct][kt][v] - from);
-          l[ct] += e;
-          p[ct][kt >> 1][4 * (kt & 1) + v] = (_Float16)e;
-        }
-    }
+        for (int v = 0; v < 4; ++v)
+          p[ct][kt >> 1][4 * (kt & 1) + v] = (_Float16)__builtin_amdgcn_exp2f(fmaf(s[ct][kt][v], sc[ct], from[ct]));
+    store_k(slot);
+    store_v(slot ^ 1);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const h8 vv = *(const h8*)(vls[slot] + (NT * c + n) * VROW + (((4 * h + g) ^ (c & 7)) * 16));
-        o[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[0][h], o[0][n], 0, 0, 0);
-        o[1][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[1][h], o[1][n], 0, 0, 0);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[ct][h], o[ct][n], 0, 0, 0);
       }
-  };
-
-  if (b0 < b1) {
-    store_block(0);
-    if (b0 + 1 < b1) load_block(b0 + 1);
-  }
-  __syncthreads();
-  for (int blk = b0; blk < b1; ++blk) {
-    const int slot = (blk - b0) & 1;
-    if (blk + 1 < b1) {                    // into the other buffer, whose readers passed the last barrier
-      store_block(slot ^ 1);
-      if (blk + 2 < b1) load_block(blk + 2);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) l[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[ct][h], l[ct], 0, 0, 0);
     }
-    compute(blk, slot);
+    load_k(blk + 3);
+    load_v(blk + 2);
     __syncthreads();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) s[ct][kt] = next[ct][kt];
   }
 
   const int64_t all = (int64_t)a.batch * a.KV * a.rows;
 #pragma unroll
-  for (int ct = 0; ct < 2; ++ct) {
-    float L = l[ct];
-    L += __shfl_xor(L, 16, 64);
-    L += __shfl_xor(L, 32, 64);
+  for (int ct = 0; ct < CT; ++ct) {
+    const float L = l[ct][0];
     const int r = w0 + 16 * ct + c;
     if (r >= a.rows) continue;
     const int t = r / a.G, hg = r - t * a.G;
     const int64_t at = sp * all + ((int64_t)b * a.KV + kvh) * a.rows + r;
     if (a.splits > 1 && g == 0) {
       float* ml = a.part + a.splits * all * D + 2 * at;
-      ml[0] = m[ct];
+      ml[0] = m[ct] * sc[ct];
       ml[1] = L;
     }
     const float inv = a.splits > 1 ? 1.f : L > 0.f ? 1.f / L : 0.f;
@@ -784,18 +845,30 @@ bool rows_aligned(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t siz
   return aligned16(p) && sb * size % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
 }
 
-// How the work of an attention call is cut: tiles of 16 query rows (few rows)
-// or of 128, and splits of their keys so that a small call still fills the card.
+// How the work of an attention call is cut: tiles of 16 query rows (few rows),
+// 64 or 128, and splits of their keys so that a small call still fills the card.
 struct Cut {
-  bool wide;
-  int tiles, splits;
+  int rows, tiles, splits;                 // query rows of a tile: 16, 64 or 128
 };
 Cut cut_of(int64_t batch, int64_t rows, int64_t KV, int64_t max_len) {
-  const bool wide = rows > 64;
-  const int64_t tile = wide ? kTileRows : 16, keys = wide ? 512 : 32 * kRowWaves;
+  const int64_t forced = tuning(BF16X_TUNE_KV4_TILE);
+  const int64_t wide = batch * KV * ((rows + 127) / 128);
+  const int64_t tile = forced == 16 || forced == 64 || forced == 128 ? forced : rows <= 64 ? 16 : wide < 256 ? 64 : 128;
+  const int64_t keys = tile > 16 ? 512 : 32 * kRowWaves;
   const int64_t tiles = (rows + tile - 1) / tile, wgs = batch * KV * tiles;
   const int64_t want = wgs > 0 ? 512 / wgs : 1, most = (max_len + keys - 1) / keys;
-  return {wide, (int)tiles, (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}))};
+  const int64_t split = tuning(BF16X_TUNE_KV4_SPLIT);
+  return {(int)tile, (int)tiles,
+          (int)std::max<int64_t>(1, std::min<int64_t>(split > 0 ? split : std::min(want, most), kMaxSplits))};
+}
+
+template <int D, bool BF>
+void launch(const AttnArgs& a, int tile_rows, int64_t blocks, int64_t out_rows, hipStream_t st) {
+  const dim3 grid((unsigned)blocks);
+  if (tile_rows == 128) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, 2, BF>), grid, dim3(256), 0, st, a);
+  else if (tile_rows == 64) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, 1, BF>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), grid, dim3(64 * kRowWaves), 0, st, a);
+  if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)out_rows), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -904,37 +977,9 @@ extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, in
              (int)max_len, (int)rows, cut.tiles, cut.splits, (int)win, scale, k_codes, (const uint32_t*)k_scales,
              v_codes, (const uint32_t*)v_scales, pos, start, (uint16_t*)out, (float*)workspace};
   const hipStream_t st = (hipStream_t)stream;
-#define ROWS(D, BF) hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), dim3((unsigned)blocks), dim3(64 * kRowWaves), 0, st, a)
-#define TILES(D, BF) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, BF>), dim3((unsigned)blocks), dim3(256), 0, st, a)
-#define JOIN(D, BF) \
-  hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)(batch * n_kv_heads * rows)), dim3(256), 0, st, a)
   const bool bf = type == BF16X_BF16;
-  if (cut.wide) {
-    if (head_dim == 128) {
-      if (bf) TILES(128, true);
-      else TILES(128, false);
-    } else {
-      if (bf) TILES(64, true);
-      else TILES(64, false);
-    }
-  } else if (head_dim == 128) {
-    if (bf) ROWS(128, true);
-    else ROWS(128, false);
-  } else {
-    if (bf) ROWS(64, true);
-    else ROWS(64, false);
-  }
-  if (cut.splits > 1) {
-    if (head_dim == 128) {
-      if (bf) JOIN(128, true);
-      else JOIN(128, false);
-    } else {
-      if (bf) JOIN(64, true);
-      else JOIN(64, false);
-    }
-  }
-#undef ROWS
-#undef TILES
-#undef JOIN
+  const int64_t out_rows = batch * n_kv_heads * rows;
+  if (head_dim == 128) bf ? launch<128, true>(a, cut.rows, blocks, out_rows, st) : launch<128, false>(a, cut.rows, blocks, out_rows, st);
+  else bf ? launch<64, true>(a, cut.rows, blocks, out_rows, st) : launch<64, false>(a, cut.rows, blocks, out_rows, st);
   return launch_status();
 }
