@@ -277,63 +277,73 @@ __device__ __forceinline__ float load_query(const uint16_t* src, bool valid, flo
   return fmaxf(fabsf(scale) * kLog2e * __uint_as_float((uint32_t)(127 + e2) << 23), 1.2e-38f);
 }
 
-// Few query rows (single tokens, drafts): a tile of 16 rows; 4 waves take the
-// 32-key steps of the workgroup's range in turn, each straight from the cache
-// into MFMA operands, with a running maximum and sum per row; the waves meet
-// in LDS once, at the end.
+// Maximum over the 4 lanes that hold a row's keys (lanes c, c + 16, c + 32, c + 48).
+__device__ __forceinline__ float row_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Few query rows (single tokens, drafts): a tile of 16 rows; the waves of a
+// workgroup take the 32-key steps of its range in turn, each straight from the
+// cache into MFMA operands, with a running maximum and sum per row, and meet in
+// LDS once, at the end.
+constexpr int kRowWaves = 8;
+
 template <int D>
 struct Step {
   static constexpr int W = D / 32;         // words of codes of a key per lane in the first product
   uint32_t kc[2][W], ks[2], vc[8], vs[8];
 };
 
-template <int D>
-__device__ __forceinline__ void load_step(Step<D>& s, const uint8_t* kc, const uint32_t* ks, const uint8_t* vc,
-                                          const uint32_t* vs, int j0, int last, int c, int g) {
+// The K and V rows of a step, from the addresses of its first.  CUT: rows past `last` are taken as that one.
+template <int D, bool CUT>
+__device__ __forceinline__ void load_k(Step<D>& s, const uint8_t* kb, const uint32_t* ks, int last, int c, int g) {
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    const int64_t j = min(j0 + 16 * kt + c, last);
+    const uint32_t j = CUT ? min(16 * kt + c, last) : 16 * kt + c;
     if constexpr (D == 128) {
-      const u32x4 w = *(const u32x4*)(kc + j * (D / 2) + 16 * g);
+      const u32x4 w = *(const u32x4*)(kb + (j * (D / 2) + 16 * g));
       s.kc[kt][0] = w.x, s.kc[kt][1] = w.y, s.kc[kt][2] = w.z, s.kc[kt][3] = w.w;
       s.ks[kt] = ks[j * (D / 32) + g];
     } else {
-      const uint2 w = *(const uint2*)(kc + j * (D / 2) + 8 * g);
+      const uint2 w = *(const uint2*)(kb + (j * (D / 2) + 8 * g));
       s.kc[kt][0] = w.x, s.kc[kt][1] = w.y;
       s.ks[kt] = ks[j * (D / 32) + (g >> 1)];
     }
   }
-  const int dw = c & (D / 8 - 1);
+}
+template <int D, bool CUT>
+__device__ __forceinline__ void load_v(Step<D>& s, const uint8_t* vb, const uint32_t* vs, int last, int c, int g) {
+  const uint32_t dw = c & (D / 8 - 1);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int64_t j = min(j0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4), last);
-    s.vc[e] = *(const uint32_t*)(vc + j * (D / 2) + 4 * dw);
+    const int k = e < 4 ? 4 * g + e : 16 + 4 * g + e - 4;
+    const uint32_t j = CUT ? min(k, last) : k;
+    s.vc[e] = *(const uint32_t*)(vb + (j * (D / 2) + 4 * dw));
     s.vs[e] = vs[j * (D / 32) + dw / 4];
   }
 }
 
-constexpr int kRowWaves = 4;
-
 template <int D, bool BF>
-__global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnArgs a) {
   constexpr int W = D / 32, NT = D / 16;   // steps of the first product, row blocks of the second
-  __shared__ float lo_[kRowWaves][16][D + 4];
-  __shared__ float lm[kRowWaves][16], ll[kRowWaves][16];
+  extern __shared__ float lds[];           // [waves][rows of the tile][D + 4], then (maximum, sum) of each
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   int id = blockIdx.x;
-  const int sp = id % a.splits;
-  id /= a.splits;
-  const int tile = id % a.tiles;
-  id /= a.tiles;
-  const int kvh = id % a.KV, b = id / a.KV;
-  const int r = 16 * tile + c;             // this lane's query row
-  const bool valid = r < a.rows;
-  const int t = min(r, a.rows - 1) / a.G, hg = min(r, a.rows - 1) - t * a.G;
-  int lo, hi, LO, HI, unused;
+  const int kvh = id % a.KV;
+  id /= a.KV;
+  const int b = id % a.batch;
+  id /= a.batch;
+  const int sp = id % a.splits, tile = id / a.splits;
+  const int nr = min(16, a.rows - 16 * tile), t0 = 16 * tile / a.G, t1 = (16 * tile + nr - 1) / a.G;
+  const int r = 16 * tile + min(c, nr - 1), t = r / a.G, hg = r - t * a.G;      // this lane's query row
+  int lo, hi, LO, HI, flo, fhi;
   key_range(a, b, t, lo, hi);
-  key_range(a, b, 16 * tile / a.G, LO, unused);
-  key_range(a, b, min(16 * tile + 15, a.rows - 1) / a.G, unused, HI);
+  key_range(a, b, t0, LO, fhi);            // keys that some row sees: LO .. HI; that every row sees: flo .. fhi
+  key_range(a, b, t1, flo, HI);
   const int base = LO & ~31;
   const int steps = HI > LO ? (HI - base + 31) >> 5 : 0;
   const int per = (steps + a.splits - 1) / a.splits;
@@ -342,121 +352,150 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
   const int64_t head = ((int64_t)b * a.KV + kvh) * a.max_len;
   const uint8_t *kc = a.kc + head * (D / 2), *vc = a.vc + head * (D / 2);
   const uint32_t *ks = a.ks + head * (D / 32), *vs = a.vs + head * (D / 32);
+  // (the addresses of a step are uniform; only the cache's last step may have to be cut)
+  auto next_k = [&](Step<D>& st, int step) {
+    const int64_t j0 = base + 32 * step;
+    if (j0 + 32 <= a.max_len) load_k<D, false>(st, kc + j0 * (D / 2), ks + j0 * (D / 32), 0, c, g);
+    else load_k<D, true>(st, kc + j0 * (D / 2), ks + j0 * (D / 32), a.max_len - 1 - (int)j0, c, g);
+  };
+  auto next_v = [&](Step<D>& st, int step) {
+    const int64_t j0 = base + 32 * step;
+    if (j0 + 32 <= a.max_len) load_v<D, false>(st, vc + j0 * (D / 2), vs + j0 * (D / 32), 0, c, g);
+    else load_v<D, true>(st, vc + j0 * (D / 2), vs + j0 * (D / 32), a.max_len - 1 - (int)j0, c, g);
+  };
 
+  // a wave's next K is requested when its K is used up, its next V when its V is: one set of registers, so that four
+  // waves fit a SIMD and cover each other's waits
+  const Exponents ex;
+  Step<D> cur;
+  int s = sp * per + w;
+  if (s < s1) {
+    next_k(cur, s);
+    next_v(cur, s);
+  }
   h8 qb[W];
   int qoff[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) qoff[i] = g * (D / 4) + 8 * i;
   const float sc =
-      load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, valid, a.scale, qb, qoff);
+      load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, c < nr, a.scale, qb, qoff);
 
-  float m = -INFINITY, l = 0.f;
-  f4 o[NT];
+  // m: the maximum that the weights are taken against, in units of the products; l: the sums of the rounded weights
+  float m = -INFINITY;
+  f4 o[NT], l = f4{0.f, 0.f, 0.f, 0.f};
+  const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
   for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
 
-  const Exponents ex;
-  Step<D> cur, next;
-  int s = sp * per + w;
-  if (s < s1) load_step<D>(cur, kc, ks, vc, vs, base + 32 * s, a.max_len - 1, c, g);
   for (; s < s1; s += kRowWaves) {
-    if (s + kRowWaves < s1)
-      load_step<D>(next, kc, ks, vc, vs, base + 32 * (s + kRowWaves), a.max_len - 1, c, g);
     const int j0 = base + 32 * s;
-    // scores of keys j0 + 16 kt + 4 g + v for row c
-    float x[8];
+    // products of keys j0 + 16 kt + 4 g + v with row c
+    f4 x[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       const h2 sc2 = scale_of(cur.ks[kt]), mn2 = minimum_of(cur.ks[kt]);
-      f4 acc = f4{0.f, 0.f, 0.f, 0.f};
+      x[kt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < W; ++i)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_values(cur.kc[kt][i], sc2, mn2, ex), qb[i], acc, 0, 0, 0);
+        x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_values(cur.kc[kt][i], sc2, mn2, ex), qb[i], x[kt], 0, 0, 0);
+    }
+    if (s + kRowWaves < s1) next_k(cur, s + kRowWaves);
+    if (!(j0 >= flo && j0 + 32 <= fhi)) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int j = j0 + 16 * kt + 4 * g + v;
-        x[4 * kt + v] = j >= lo && j < hi ? acc[v] * sc : -INFINITY;
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int j = j0 + 16 * kt + 4 * g + v;
+          x[kt][v] = ((j >= lo) & (j < hi)) ? x[kt][v] : -INFINITY;
+        }
+      // keys that no row of the tile sees have value 0, whatever their scales hold
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+        cur.vs[e] = ((j >= LO) & (j < HI)) ? cur.vs[e] : 0u;
       }
     }
-    float mb = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
-    mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
-    const float mn = fmaxf(m, mb);
-    const float from = mn == -INFINITY ? 0.f : mn;               // no key seen yet: every weight is 0
-    const float alpha = __builtin_amdgcn_exp2f(m - from);
-    m = mn;
-    float ps = 0.f;
+    const float mb = row_max(fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                                   fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))));
+    // weights may grow to 2^8 of the maximum that they are taken against before it is renewed (fp32 sums, and 2^8 is
+    // well inside fp16): most steps leave the outputs unscaled
+    if (__any((mb - m) * sc > 8.f)) {
+      const float mn = fmaxf(m, mb);
+      const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * sc);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n] *= alpha;
+    }
+    const float from = m == -INFINITY ? 0.f : -m * sc;           // no key seen yet: every weight is 0
     h8 pb;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float e = __builtin_amdgcn_exp2f(x[k] - from);
-      ps += e;
-      pb[k] = (_Float16)e;
-    }
-    l = l * alpha + ps;
-    // O^T += V^T P^T; keys that no row of the tile sees have value 0
-    uint32_t vsm[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = j0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
-      vsm[e] = j >= LO && j < HI ? cur.vs[e] : 0u;
-    }
-    u32x4 av[NT];
+    for (int k = 0; k < 8; ++k) pb[k] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[k >> 2][k & 3], sc, from));
+    l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, l, 0, 0, 0);
+    // O^T += V^T P^T
+    h2 s2[4], m2[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const h2 s2 = as_h2(__builtin_amdgcn_perm(vsm[2 * k + 1], vsm[2 * k], 0x05040100u));
-      const h2 m2 = as_h2(__builtin_amdgcn_perm(vsm[2 * k + 1], vsm[2 * k], 0x07060302u));
-      uint32_t va = cur.vc[2 * k], vb = cur.vc[2 * k + 1];
-      if constexpr (D == 64) {             // lanes 8 .. 15 take the upper nibbles of the same words
-        va = c & 8 ? va >> 16 : va;
-        vb = c & 8 ? vb >> 16 : vb;
-      }
+      s2[k] = as_h2(__builtin_amdgcn_perm(cur.vs[2 * k + 1], cur.vs[2 * k], 0x05040100u));
+      m2[k] = as_h2(__builtin_amdgcn_perm(cur.vs[2 * k + 1], cur.vs[2 * k], 0x07060302u));
+    }
+    if constexpr (D == 64) {               // lanes 8 .. 15 take the upper nibbles of the same words
 #pragma unroll
-      for (int y = 0; y < NT / 2; ++y) {
-        const uint32_t two = __builtin_amdgcn_perm(vb, va, 0x0C040C00u + 0x00010001u * y);
-        av[2 * y][k] = as_u32(__builtin_elementwise_fma(low_codes(two, ex), s2, m2));
-        av[2 * y + 1][k] = as_u32(__builtin_elementwise_fma(high_codes(two, ex), s2, m2));
-      }
+      for (int e = 0; e < 8; ++e) cur.vc[e] = c & 8 ? cur.vc[e] >> 16 : cur.vc[e];
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      o[n] *= alpha;
-      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, av[n]), pb, o[n], 0, 0, 0);
+    for (int y = 0; y < NT / 2; ++y) {
+      u32x4 va, vb;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t two = __builtin_amdgcn_perm(cur.vc[2 * k + 1], cur.vc[2 * k], 0x0C040C00u + 0x00010001u * y);
+        va[k] = as_u32(__builtin_elementwise_fma(low_codes(two, ex), s2[k], m2[k]));
+        vb[k] = as_u32(__builtin_elementwise_fma(high_codes(two, ex), s2[k], m2[k]));
+      }
+      o[2 * y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, va), pb, o[2 * y], 0, 0, 0);
+      o[2 * y + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vb), pb, o[2 * y + 1], 0, 0, 0);
     }
-    cur = next;
+    if (s + kRowWaves < s1) next_v(cur, s + kRowWaves);
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
 
   // the waves' results meet: row c, dims of D row 4 g + v and row block n
+  float* lml = lds + kRowWaves * nr * (D + 4);
+  if (c < nr) {
+    float* to = lds + (w * nr + c) * (D + 4);
 #pragma unroll
-  for (int v = 0; v < 4; ++v)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int v = 0; v < 4; ++v) {
       const int rr = 4 * g + v;
-      // nibble n (upper nibbles for rows 8 .. 15 where D is 64) of a word: value 2 n below 4, else 2 n - 7
-      const int nib = D == 128 ? n : n + 4 * (rr >> 3);
-      const int dim = 8 * (D == 128 ? rr : rr & 7) + (nib < 4 ? 2 * nib : 2 * nib - 7);
-      lo_[w][c][dim] = o[n][v];
+      if constexpr (D == 128) {            // nibbles 0 .. 7 are values 0, 2, 4, 6, 1, 3, 5, 7 of word rr
+        *(f4*)(to + 8 * rr) = f4{o[0][v], o[4][v], o[1][v], o[5][v]};
+        *(f4*)(to + 8 * rr + 4) = f4{o[2][v], o[6][v], o[3][v], o[7][v]};
+      } else {                             // rows 8 .. 15 hold the upper nibbles
+#pragma unroll
+        for (int n = 0; n < NT; ++n) to[8 * (rr & 7) + 2 * n + (rr >> 3)] = o[n][v];
+      }
     }
-  if (g == 0) lm[w][c] = m, ll[w][c] = l;
+    if (g == 0) {
+      lml[2 * (w * nr + c)] = m * sc;
+      lml[2 * (w * nr + c) + 1] = l[0];
+    }
+  }
   __syncthreads();
   constexpr int E = 16 * D / (64 * kRowWaves);                  // values of the tile per thread
   const int rr = tid / (D / E), d0 = tid % (D / E) * E;
+  if (rr >= nr) return;
   const int R = 16 * tile + rr;
-  if (R >= a.rows) return;
-  float M = lm[0][rr];
+  float M = lml[2 * rr];
 #pragma unroll
-  for (int u = 1; u < kRowWaves; ++u) M = fmaxf(M, lm[u][rr]);
+  for (int u = 1; u < kRowWaves; ++u) M = fmaxf(M, lml[2 * (u * nr + rr)]);
+  const float from = M == -INFINITY ? 0.f : M;
   float L = 0.f, y[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) y[e] = 0.f;
 #pragma unroll
   for (int u = 0; u < kRowWaves; ++u) {
-    const float f = lm[u][rr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lm[u][rr] - M);
-    L = fmaf(ll[u][rr], f, L);
+    const float f = __builtin_amdgcn_exp2f(lml[2 * (u * nr + rr)] - from);
+    L = fmaf(lml[2 * (u * nr + rr) + 1], f, L);
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = fmaf(lo_[u][rr][d0 + e], f, y[e]);
+    for (int e = 0; e < E; ++e) y[e] = fmaf(lds[(u * nr + rr) * (D + 4) + d0 + e], f, y[e]);
   }
   if (a.splits == 1) {
     const float inv = L > 0.f ? 1.f / L : 0.f;
@@ -486,14 +525,6 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv4_attn_rows_kernel(AttnArgs 
 // product n.  Two buffers, one barrier per block; the next block's codes are in
 // registers while this one is multiplied.
 constexpr int kBlock = 64;                 // keys
-
-// Maximum over the 4 lanes that hold a row's keys (lanes c, c + 16, c + 32, c + 48).
-__device__ __forceinline__ float row_max(float x) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
 
 template <int D, int CT, bool BF>
 __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
@@ -867,7 +898,8 @@ void launch(const AttnArgs& a, int tile_rows, int64_t blocks, int64_t out_rows, 
   const dim3 grid((unsigned)blocks);
   if (tile_rows == 128) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, 2, BF>), grid, dim3(256), 0, st, a);
   else if (tile_rows == 64) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, 1, BF>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), grid, dim3(64 * kRowWaves), 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), grid, dim3(64 * kRowWaves),
+                          (size_t)kRowWaves * std::min(16, a.rows) * (D + 6) * 4, st, a);
   if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)out_rows), dim3(256), 0, st, a);
 }
 
