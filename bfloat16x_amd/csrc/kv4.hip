@@ -26,6 +26,7 @@ using namespace bf16x;
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLargest = 61440.f;       // 15 x 4096: minimum + 15 scale stays an fp16 number whatever was rounded
 constexpr float kLog2e = 1.44269504088896341f;
@@ -63,25 +64,29 @@ __device__ __forceinline__ h2 minimum_of(uint32_t w) { return as_h2(__builtin_am
 // row; the 4 lanes of a group meet in two quad exchanges.
 
 template <int TYPE>
+__device__ __forceinline__ void values8(u32x4 r, float (&x)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (TYPE == BF16X_BF16) {
+      x[2 * e] = bf16lo_to_f32(w[e]);
+      x[2 * e + 1] = bf16hi_to_f32(w[e]);
+    } else {
+      const h2 h = as_h2(w[e]);
+      x[2 * e] = (float)h.x;
+      x[2 * e + 1] = (float)h.y;
+    }
+  }
+}
+
+template <int TYPE>
 __device__ __forceinline__ void load8(const void* p, int64_t i, float (&x)[8]) {
   if constexpr (TYPE == BF16X_F32) {
     const f4 a = *(const f4*)((const float*)p + i), b = *(const f4*)((const float*)p + i + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
   } else {
-    const u32x4 r = *(const u32x4*)((const uint16_t*)p + i);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (TYPE == BF16X_BF16) {
-        x[2 * e] = bf16lo_to_f32(w[e]);
-        x[2 * e + 1] = bf16hi_to_f32(w[e]);
-      } else {
-        const h2 h = as_h2(w[e]);
-        x[2 * e] = (float)h.x;
-        x[2 * e + 1] = (float)h.y;
-      }
-    }
+    values8<TYPE>(*(const u32x4*)((const uint16_t*)p + i), x);
   }
 }
 
@@ -222,6 +227,7 @@ struct AttnArgs {
   int tiles, splits;
   int window;                              // 0: none
   float scale;
+  uint32_t g_inv;                          // 2^32 / G, rounded up
   const uint8_t* kc;
   const uint32_t* ks;
   const uint8_t* vc;
@@ -230,6 +236,16 @@ struct AttnArgs {
   uint16_t* out;
   float* part;                             // [splits][batch KV rows][D] unnormalised outputs, then [..][2] (max, sum)
 };
+
+// Token of a query row.
+__device__ __forceinline__ int token_of(const AttnArgs& a, int r) {
+  if (a.G == 1) return r;
+  const int t = (int)__umulhi((uint32_t)r, a.g_inv);            // at most one too many for r < 2^30
+  return t * a.G > r ? t - 1 : t;
+}
+
+// A value that is the same in every lane, known to the compiler as such.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Keys [lo, hi) that the query at token t sees.
 __device__ __forceinline__ void key_range(const AttnArgs& a, int b, int t, int& lo, int& hi) {
@@ -247,33 +263,41 @@ __device__ __forceinline__ uint32_t out2(float a, float b) {
   return BF ? f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16) : as_u32(h2{(_Float16)a, (_Float16)b});
 }
 
-// The query operand of a lane: NW words of 2 values at `src` brought to fp16
-// by the power of two that puts the row's largest value (over the 4 lanes of
+// The query operand of a lane: 8 N values of its row brought to fp16 by the power of two that puts the row's largest value (over the 4 lanes of
 // the row) into [1, 2), with the sign of `scale`; returns what a product's sum
 // is to be multiplied with for a score in powers of two, a positive number.
 // Exact for every value within 2^-14 of the row's largest.
 template <bool BF, int N>
-__device__ __forceinline__ float load_query(const uint16_t* src, bool valid, float scale, h8 (&qb)[N],
-                                            const int (&off)[N]) {
-  float x[N][8];
-  float mx = 0.f;
+__device__ __forceinline__ float load_query(const u32x4 (&raw)[N], bool valid, float scale, h8 (&qb)[N]) {
+  us2 big = {0, 0};                        // largest magnitude as bits: ascending for both types
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-    if (valid) load8<BF ? BF16X_BF16 : BF16X_F16>(src, off[i], x[i]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
-  }
-  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-  int e2 = (int)(__float_as_uint(mx) >> 23) - 127;
-  e2 = mx > 0.f && e2 < 128 ? max(e2, -100) : 0;
+    for (int e = 0; e < 4; ++e)
+      big = __builtin_elementwise_max(big, __builtin_bit_cast(us2, raw[i][e] & 0x7FFF7FFFu));
+  uint32_t mx = valid ? max(big.x, big.y) : 0;
+  mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, 64));
+  mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, 64));
+  const uint32_t bits = BF ? mx << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)mx));
+  int e2 = (int)(bits >> 23) - 127;        // (infinities and NaN keep their row as it is)
+  e2 = mx > 0 && e2 < 128 ? max(e2, -100) : 0;
   const float down = copysignf(__uint_as_float((uint32_t)(127 - e2) << 23), scale);
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) qb[i][e] = (_Float16)(x[i][e] * down);
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = valid ? raw[i][e] : 0u;
+      float x, y;
+      if constexpr (BF) {
+        x = bf16lo_to_f32(w);
+        y = bf16hi_to_f32(w);
+      } else {
+        x = (float)as_h2(w).x;
+        y = (float)as_h2(w).y;
+      }
+      qb[i][2 * e] = (_Float16)(x * down);
+      qb[i][2 * e + 1] = (_Float16)(y * down);
+    }
   return fmaxf(fabsf(scale) * kLog2e * __uint_as_float((uint32_t)(127 + e2) << 23), 1.2e-38f);
 }
 
@@ -288,8 +312,9 @@ __device__ __forceinline__ float row_max(float x) {
 // Few query rows (single tokens, drafts): a tile of 16 rows; the waves of a
 // workgroup take the 32-key steps of its range in turn, each straight from the
 // cache into MFMA operands, with a running maximum and sum per row, and meet in
-// LDS once, at the end.
+// LDS once, at the end.  At 128 registers two workgroups fit a CU.
 constexpr int kRowWaves = 8;
+constexpr int kRowGroups = 1024;           // workgroups with keys that a batch's work is cut into
 
 template <int D>
 struct Step {
@@ -297,71 +322,115 @@ struct Step {
   uint32_t kc[2][W], ks[2], vc[8], vs[8];
 };
 
-// The K and V rows of a step, from the addresses of its first.  CUT: rows past `last` are taken as that one.
-template <int D, bool CUT>
-__device__ __forceinline__ void load_k(Step<D>& s, const uint8_t* kb, const uint32_t* ks, int last, int c, int g) {
+// A lane's byte offsets in a step's rows, opaque to the compiler: the loads of
+// a step are then a uniform address, one of these and a constant, where it
+// would keep a 64-bit address of every load in registers.
+template <int D>
+struct Offsets {
+  uint32_t k, ks, v, vs;
+  __device__ __forceinline__ Offsets(int c, int g) {
+    const int dw = c & (D / 8 - 1);
+    k = c * (D / 2) + g * (D / 8);
+    ks = 4 * (c * (D / 32) + (D == 128 ? g : g >> 1));
+    v = 4 * g * (D / 2) + 4 * dw;
+    vs = 4 * (4 * g * (D / 32) + dw / 4);
+    asm("" : "+v"(k), "+v"(ks), "+v"(v), "+v"(vs));
+  }
+};
+template <class T>
+__device__ __forceinline__ T load_at(const void* p, uint32_t off, int more) {
+  return *(const T*)((const char*)p + off + more);
+}
+
+// The K and V rows of a step, from the addresses of its first.  SHORT: rows past `last` are taken as that one.
+template <int D, bool SHORT>
+__device__ __forceinline__ void load_k(Step<D>& s, const void* kb, const void* ks, int last, const Offsets<D>& o, int c) {
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    const uint32_t j = CUT ? min(16 * kt + c, last) : 16 * kt + c;
+    const int up = SHORT ? min(16 * kt + c, last) - c : 16 * kt;
     if constexpr (D == 128) {
-      const u32x4 w = *(const u32x4*)(kb + (j * (D / 2) + 16 * g));
+      const u32x4 w = load_at<u32x4>(kb, o.k, up * (D / 2));
       s.kc[kt][0] = w.x, s.kc[kt][1] = w.y, s.kc[kt][2] = w.z, s.kc[kt][3] = w.w;
-      s.ks[kt] = ks[j * (D / 32) + g];
     } else {
-      const uint2 w = *(const uint2*)(kb + (j * (D / 2) + 8 * g));
+      const uint2 w = load_at<uint2>(kb, o.k, up * (D / 2));
       s.kc[kt][0] = w.x, s.kc[kt][1] = w.y;
-      s.ks[kt] = ks[j * (D / 32) + (g >> 1)];
     }
+    s.ks[kt] = load_at<uint32_t>(ks, o.ks, up * (D / 8));
   }
 }
-template <int D, bool CUT>
-__device__ __forceinline__ void load_v(Step<D>& s, const uint8_t* vb, const uint32_t* vs, int last, int c, int g) {
-  const uint32_t dw = c & (D / 8 - 1);
+template <int D, bool SHORT>
+__device__ __forceinline__ void load_v(Step<D>& s, const void* vb, const void* vs, int last, const Offsets<D>& o, int g) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int k = e < 4 ? 4 * g + e : 16 + 4 * g + e - 4;
-    const uint32_t j = CUT ? min(k, last) : k;
-    s.vc[e] = *(const uint32_t*)(vb + (j * (D / 2) + 4 * dw));
-    s.vs[e] = vs[j * (D / 32) + dw / 4];
+    const int k = e < 4 ? e : 12 + e;
+    const int up = SHORT ? min(4 * g + k, last) - 4 * g : k;
+    s.vc[e] = load_at<uint32_t>(vb, o.v, up * (D / 2));
+    s.vs[e] = load_at<uint32_t>(vs, o.vs, up * (D / 8));
   }
 }
 
-template <int D, bool BF>
-__global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnArgs a) {
+// SHORT: a cache of fewer than 32 rows; otherwise the step that would pass the
+// cache's end takes its last 32 rows and hides those of the step before.
+template <int D, bool SHORT, bool BF>
+__global__ __launch_bounds__(64 * kRowWaves, SHORT ? 2 : 4) void kv4_attn_rows_kernel(AttnArgs a) {
   constexpr int W = D / 32, NT = D / 16;   // steps of the first product, row blocks of the second
   extern __shared__ float lds[];           // [waves][rows of the tile][D + 4], then (maximum, sum) of each
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int id = blockIdx.x;
-  const int kvh = id % a.KV;
-  id /= a.KV;
-  const int b = id % a.batch;
-  id /= a.batch;
-  const int sp = id % a.splits, tile = id / a.splits;
-  const int nr = min(16, a.rows - 16 * tile), t0 = 16 * tile / a.G, t1 = (16 * tile + nr - 1) / a.G;
-  const int r = 16 * tile + min(c, nr - 1), t = r / a.G, hg = r - t * a.G;      // this lane's query row
-  int lo, hi, LO, HI, flo, fhi;
+  const int kvh = blockIdx.x, b = blockIdx.z;
+  const int sp = a.tiles == 1 ? blockIdx.y : blockIdx.y % a.splits, tile = a.tiles == 1 ? 0 : blockIdx.y / a.splits;
+  const int nr = min(16, a.rows - 16 * tile);
+  const int r = 16 * tile + min(c, nr - 1), t = token_of(a, r), hg = r - t * a.G;       // this lane's query row
+  const int t0 = token_of(a, 16 * tile), t1 = token_of(a, 16 * tile + nr - 1);
+  h8 qb[W];
+  u32x4 raw[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i)
+    raw[i] = *(const u32x4*)(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh + g * (D / 4) + 8 * i);
+  int lo, hi, LO, HI, flo, fhi, unused;
   key_range(a, b, t, lo, hi);
   key_range(a, b, t0, LO, fhi);            // keys that some row sees: LO .. HI; that every row sees: flo .. fhi
   key_range(a, b, t1, flo, HI);
+  LO = uniform(LO), HI = uniform(HI), flo = uniform(flo), fhi = uniform(fhi);
   const int base = LO & ~31;
   const int steps = HI > LO ? (HI - base + 31) >> 5 : 0;
-  const int per = (steps + a.splits - 1) / a.splits;
+  // steps per split: as many for every sequence of a batch, whose lengths differ, so that the workgroups are alike
+  int per = (steps + a.splits - 1) / a.splits;
+  if (a.splits > 1 && a.batch > 1) {
+    float total = 0.f;
+    for (int i = lane; i < a.batch; i += 64) {
+      int l0, h1;
+      key_range(a, i, t0, l0, unused);
+      key_range(a, i, t1, unused, h1);
+      total += (float)(max(h1 - l0, 0) >> 5) + 1.f;
+    }
+    const float share = wave_sum(total) * (float)(a.KV * a.tiles) / kRowGroups;
+    per = max(per, uniform((int)fminf(share, 1e9f)));
+  }
   const int s1 = min((sp + 1) * per, steps);
+  if (sp * per >= steps && a.splits > 1) { // nothing left for this split
+    if (tid < nr) {
+      const int64_t all = (int64_t)a.batch * a.KV * a.rows;
+      float* ml = a.part + a.splits * all * D +
+                  2 * (sp * all + ((int64_t)b * a.KV + kvh) * a.rows + 16 * tile + tid);
+      ml[0] = -INFINITY;
+      ml[1] = 0.f;
+    }
+    return;
+  }
 
   const int64_t head = ((int64_t)b * a.KV + kvh) * a.max_len;
   const uint8_t *kc = a.kc + head * (D / 2), *vc = a.vc + head * (D / 2);
   const uint32_t *ks = a.ks + head * (D / 32), *vs = a.vs + head * (D / 32);
-  // (the addresses of a step are uniform; only the cache's last step may have to be cut)
+  const Offsets<D> off(c, g);
+  auto first_row = [&](int step) { return SHORT ? 0 : min(base + 32 * step, a.max_len - 32); };
   auto next_k = [&](Step<D>& st, int step) {
-    const int64_t j0 = base + 32 * step;
-    if (j0 + 32 <= a.max_len) load_k<D, false>(st, kc + j0 * (D / 2), ks + j0 * (D / 32), 0, c, g);
-    else load_k<D, true>(st, kc + j0 * (D / 2), ks + j0 * (D / 32), a.max_len - 1 - (int)j0, c, g);
+    const int64_t j = first_row(step);
+    load_k<D, SHORT>(st, kc + j * (D / 2), ks + j * (D / 32), a.max_len - 1, off, c);
   };
   auto next_v = [&](Step<D>& st, int step) {
-    const int64_t j0 = base + 32 * step;
-    if (j0 + 32 <= a.max_len) load_v<D, false>(st, vc + j0 * (D / 2), vs + j0 * (D / 32), 0, c, g);
-    else load_v<D, true>(st, vc + j0 * (D / 2), vs + j0 * (D / 32), a.max_len - 1 - (int)j0, c, g);
+    const int64_t j = first_row(step);
+    load_v<D, SHORT>(st, vc + j * (D / 2), vs + j * (D / 32), a.max_len - 1, off, g);
   };
 
   // a wave's next K is requested when its K is used up, its next V when its V is: one set of registers, so that four
@@ -373,23 +442,18 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnAr
     next_k(cur, s);
     next_v(cur, s);
   }
-  h8 qb[W];
-  int qoff[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) qoff[i] = g * (D / 4) + 8 * i;
-  const float sc =
-      load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, c < nr, a.scale, qb, qoff);
+  const float sc = load_query<BF>(raw, c < nr, a.scale, qb);
 
-  // m: the maximum that the weights are taken against, in units of the products; l: the sums of the rounded weights
-  float m = -INFINITY;
-  f4 o[NT], l = f4{0.f, 0.f, 0.f, 0.f};
-  const h8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+  // m: the maximum that the weights are taken against, in units of the products; l: the lane's part of
+  // their sum
+  float m = -INFINITY, l = 0.f;
+  f4 o[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) o[n] = f4{0.f, 0.f, 0.f, 0.f};
 
   for (; s < s1; s += kRowWaves) {
-    const int j0 = base + 32 * s;
-    // products of keys j0 + 16 kt + 4 g + v with row c
+    const int j0 = base + 32 * s, jb = first_row(s);
+    // products of keys jb + 16 kt + 4 g + v with row c
     f4 x[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -405,14 +469,14 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnAr
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int j = j0 + 16 * kt + 4 * g + v;
-          x[kt][v] = ((j >= lo) & (j < hi)) ? x[kt][v] : -INFINITY;
+          const int j = jb + 16 * kt + 4 * g + v;
+          x[kt][v] = ((j >= max(lo, j0)) & (j < hi)) ? x[kt][v] : -INFINITY;
         }
       // keys that no row of the tile sees have value 0, whatever their scales hold
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int j = j0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
-        cur.vs[e] = ((j >= LO) & (j < HI)) ? cur.vs[e] : 0u;
+        const int j = jb + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+        cur.vs[e] = ((j >= max(LO, j0)) & (j < HI)) ? cur.vs[e] : 0u;
       }
     }
     const float mb = row_max(fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
@@ -430,8 +494,11 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnAr
     const float from = m == -INFINITY ? 0.f : -m * sc;           // no key seen yet: every weight is 0
     h8 pb;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) pb[k] = (_Float16)__builtin_amdgcn_exp2f(fmaf(x[k >> 2][k & 3], sc, from));
-    l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, l, 0, 0, 0);
+    for (int k = 0; k < 8; ++k) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(x[k >> 2][k & 3], sc, from));
+      l += e;
+      pb[k] = (_Float16)e;
+    }
     // O^T += V^T P^T
     h2 s2[4], m2[4];
 #pragma unroll
@@ -458,6 +525,9 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnAr
     if (s + kRowWaves < s1) next_v(cur, s + kRowWaves);
   }
 
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+
   // the waves' results meet: row c, dims of D row 4 g + v and row block n
   float* lml = lds + kRowWaves * nr * (D + 4);
   if (c < nr) {
@@ -475,7 +545,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnAr
     }
     if (g == 0) {
       lml[2 * (w * nr + c)] = m * sc;
-      lml[2 * (w * nr + c) + 1] = l[0];
+      lml[2 * (w * nr + c) + 1] = l;
     }
   }
   __syncthreads();
@@ -499,7 +569,7 @@ __global__ __launch_bounds__(64 * kRowWaves, 4) void kv4_attn_rows_kernel(AttnAr
   }
   if (a.splits == 1) {
     const float inv = L > 0.f ? 1.f / L : 0.f;
-    const int tt = R / a.G, hh = R - tt * a.G;
+    const int tt = token_of(a, R), hh = R - tt * a.G;
     uint32_t* op = (uint32_t*)(a.out + (((int64_t)b * a.tokens + tt) * a.H + kvh * a.G + hh) * D + d0);
 #pragma unroll
     for (int e = 0; e < E; e += 2) op[e / 2] = out2<BF>(y[e] * inv, y[e + 1] * inv);
@@ -537,20 +607,17 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads fastest, so that a head's tiles share an XCD's L2 where there are 8; the last tiles, which see the most
   // keys, first
-  int id = blockIdx.x;
-  const int kvh = id % a.KV;
-  id /= a.KV;
-  const int b = id % a.batch;
-  id /= a.batch;
-  const int sp = id % a.splits, tile = a.tiles - 1 - id / a.splits;
+  const int kvh = blockIdx.x, b = blockIdx.z;
+  const int sp = a.splits == 1 ? 0 : blockIdx.y % a.splits, tile = a.tiles - 1 - (a.splits == 1 ? blockIdx.y : blockIdx.y / a.splits);
   const int r0 = kTileRows * tile, w0 = r0 + 16 * CT * w;
   int lo[CT], hi[CT], LO, HI, flo = 0, fhi = 0, unused;
-  key_range(a, b, r0 / a.G, LO, unused);
-  key_range(a, b, min(r0 + kTileRows - 1, a.rows - 1) / a.G, unused, HI);
+  key_range(a, b, token_of(a, r0), LO, unused);
+  key_range(a, b, token_of(a, min(r0 + kTileRows - 1, a.rows - 1)), unused, HI);
   if (w0 < a.rows) {                       // keys that every row of the wave sees
-    key_range(a, b, w0 / a.G, unused, fhi);
-    key_range(a, b, min(w0 + 16 * CT - 1, a.rows - 1) / a.G, flo, unused);
+    key_range(a, b, token_of(a, w0), unused, fhi);
+    key_range(a, b, token_of(a, min(w0 + 16 * CT - 1, a.rows - 1)), flo, unused);
   }
+  LO = uniform(LO), HI = uniform(HI), flo = uniform(flo), fhi = uniform(fhi);
   const int base = LO & ~(kBlock - 1);
   const int blocks = HI > LO ? (HI - base + kBlock - 1) / kBlock : 0;
   const int per = (blocks + a.splits - 1) / a.splits;
@@ -639,15 +706,15 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   }
   h8 qb[CT][W];
   float sc[CT];
-  int qoff[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) qoff[i] = 32 * i + 8 * g;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int r = w0 + 16 * ct + c, rc = min(r, a.rows - 1), t = rc / a.G, hg = rc - t * a.G;
+    const int r = w0 + 16 * ct + c, rc = min(r, a.rows - 1), t = token_of(a, rc), hg = rc - t * a.G;
     key_range(a, b, t, lo[ct], hi[ct]);
-    sc[ct] = load_query<BF>(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh, r < a.rows, a.scale, qb[ct],
-                            qoff);
+    u32x4 raw[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      raw[i] = *(const u32x4*)(a.q + b * a.q_sb + t * a.q_st + (kvh * a.G + hg) * a.q_sh + 32 * i + 8 * g);
+    sc[ct] = load_query<BF>(raw, r < a.rows, a.scale, qb[ct]);
   }
   // m: the maximum that the weights are taken against, in units of the products; l: their sums, from the same
   // rounded weights as the outputs (a product with ones: all four registers hold the row's sum)
@@ -766,7 +833,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
     const float L = l[ct][0];
     const int r = w0 + 16 * ct + c;
     if (r >= a.rows) continue;
-    const int t = r / a.G, hg = r - t * a.G;
+    const int t = token_of(a, r), hg = r - t * a.G;
     const int64_t at = sp * all + ((int64_t)b * a.KV + kvh) * a.rows + r;
     if (a.splits > 1 && g == 0) {
       float* ml = a.part + a.splits * all * D + 2 * at;
@@ -810,7 +877,8 @@ template <int D, bool BF>
 __global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a) {
   constexpr int LS = D / 4, NG = 256 / LS, E = kMaxSplits / NG;
   __shared__ f4 sum[NG][LS];
-  const int64_t all = (int64_t)a.batch * a.KV * a.rows, at = blockIdx.x;
+  const int64_t all = (int64_t)a.batch * a.KV * a.rows;
+  const int64_t at = ((int64_t)blockIdx.z * a.KV + blockIdx.y) * a.rows + blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, grp = tid / LS, d = tid % LS;
   const float* ml = a.part + a.splits * all * D;
   float mv[kMaxSplits / 64], lv[kMaxSplits / 64], M = -INFINITY, L = 0.f;
@@ -841,17 +909,16 @@ __global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int s = grp + NG * e;
-    y += v[e] * __shfl(f[NG * e / 64], s & 63, 64);
+    const float fe = __shfl(f[NG * e / 64], s & 63, 64);
+    y += fe > 0.f ? v[e] * fe : f4{0.f, 0.f, 0.f, 0.f};        // (an empty split's outputs are not written)
   }
   sum[grp][d] = y;
   __syncthreads();
   if (grp) return;
 #pragma unroll
   for (int k = 1; k < NG; ++k) y += sum[k][d];
-  const int64_t bk = at / a.rows;
-  const int r = (int)(at - bk * a.rows), t = r / a.G, hg = r - t * a.G;
-  const int64_t b = bk / a.KV;
-  const int kvh = (int)(bk - b * a.KV);
+  const int r = blockIdx.x, t = token_of(a, r), hg = r - t * a.G, kvh = blockIdx.y;
+  const int64_t b = blockIdx.z;
   y *= L > 0.f ? 1.f / L : 0.f;
   *(uint2*)(a.out + ((b * a.tokens + t) * a.H + kvh * a.G + hg) * D + 4 * d) =
       make_uint2(out2<BF>(y[0], y[1]), out2<BF>(y[2], y[3]));
@@ -879,28 +946,34 @@ bool rows_aligned(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t siz
 // How the work of an attention call is cut: tiles of 16 query rows (few rows),
 // 64 or 128, and splits of their keys so that a small call still fills the card.
 struct Cut {
-  int rows, tiles, splits;                 // query rows of a tile: 16, 64 or 128
+  int rows, tiles, splits;
 };
-Cut cut_of(int64_t batch, int64_t rows, int64_t KV, int64_t max_len) {
-  const int64_t forced = tuning(BF16X_TUNE_KV4_TILE);
+Cut cut_of(int64_t batch, int64_t rows, int64_t tokens, int64_t KV, int64_t max_len, int64_t window) {
+  const int64_t forced = tuning(BF16X_TUNE_KV4_TILE), split = tuning(BF16X_TUNE_KV4_SPLIT);
   const int64_t wide = batch * KV * ((rows + 127) / 128);
-  const int64_t tile = forced == 16 || forced == 64 || forced == 128 ? forced : rows <= 64 ? 16 : wide < 256 ? 64 : 128;
-  const int64_t keys = tile > 16 ? 512 : 32 * kRowWaves;
-  const int64_t tiles = (rows + tile - 1) / tile, wgs = batch * KV * tiles;
-  const int64_t want = wgs > 0 ? 512 / wgs : 1, most = (max_len + keys - 1) / keys;
-  const int64_t split = tuning(BF16X_TUNE_KV4_SPLIT);
-  return {(int)tile, (int)tiles,
-          (int)std::max<int64_t>(1, std::min<int64_t>(split > 0 ? split : std::min(want, most), kMaxSplits))};
+  const int64_t tile = forced == 16 || forced == 64 || forced == 128 ? forced
+                       : rows <= 64                                  ? 16
+                       : wide < 256                                  ? 64
+                                                                     : 128;
+  const int64_t keys = window > 0 ? std::min(max_len, window + tokens) : max_len;
+  const int64_t tiles = (rows + tile - 1) / tile, wgs = std::max<int64_t>(batch * KV * tiles, 1);
+  int64_t want = std::min(tile == 16 ? 2048 / wgs : 512 / wgs, (keys + 511) / 512);
+  if (tile == 16 && keys <= 1536) want = 1;
+  if (split > 0) want = split;
+  want = std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
+  return {(int)tile, (int)tiles, (int)want};
 }
 
 template <int D, bool BF>
-void launch(const AttnArgs& a, int tile_rows, int64_t blocks, int64_t out_rows, hipStream_t st) {
-  const dim3 grid((unsigned)blocks);
+void launch(const AttnArgs& a, int tile_rows, hipStream_t st) {
+  const dim3 grid((unsigned)a.KV, (unsigned)(a.tiles * a.splits), (unsigned)a.batch);
   if (tile_rows == 128) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, 2, BF>), grid, dim3(256), 0, st, a);
   else if (tile_rows == 64) hipLaunchKernelGGL((kv4_attn_tiles_kernel<D, 1, BF>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((kv4_attn_rows_kernel<D, BF>), grid, dim3(64 * kRowWaves),
-                          (size_t)kRowWaves * std::min(16, a.rows) * (D + 6) * 4, st, a);
-  if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)out_rows), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((a.max_len < 32 ? kv4_attn_rows_kernel<D, true, BF> : kv4_attn_rows_kernel<D, false, BF>), grid,
+                          dim3(64 * kRowWaves), (size_t)kRowWaves * std::min(16, a.rows) * (D + 6) * 4, st, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((kv4_attn_join_kernel<D, BF>), dim3((unsigned)a.rows, (unsigned)a.KV, (unsigned)a.batch),
+                       dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -978,7 +1051,7 @@ extern "C" int64_t bf16x_kv4_attention_workspace(int64_t batch, int64_t tokens, 
                                                  int64_t head_dim, int64_t max_len) {
   if (check_cache(batch, tokens, n_kv_heads, head_dim, max_len) || n_heads <= 0 || n_heads % n_kv_heads) return -1;
   const int64_t rows = tokens * (n_heads / n_kv_heads);
-  const Cut cut = cut_of(batch, rows, n_kv_heads, max_len);
+  const Cut cut = cut_of(batch, rows, tokens, n_kv_heads, max_len, 0);       // (a window leaves fewer)
   return cut.splits == 1 ? 0 : cut.splits * batch * n_kv_heads * rows * (head_dim + 2) * 4;
 }
 
@@ -1000,18 +1073,16 @@ extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, in
   if (need > 0 && (!workspace || workspace_bytes < need)) return BF16X_ECAPACITY;
   if (batch == 0 || tokens == 0) return BF16X_OK;
   const int64_t G = n_heads / n_kv_heads, rows = tokens * G;
-  const Cut cut = cut_of(batch, rows, n_kv_heads, max_len);
-  const int64_t blocks = batch * n_kv_heads * cut.tiles * cut.splits;
-  if (rows > 0x3FFFFFFF || blocks > 0x7FFFFFFF || batch * n_kv_heads * rows > 0x7FFFFFFF) return BF16X_ESHAPE;
+  const Cut cut = cut_of(batch, rows, tokens, n_kv_heads, max_len, window);
+  if (rows > 0x3FFFFFFF || (int64_t)cut.tiles * cut.splits > 65535 || batch > 65535) return BF16X_ESHAPE;
   // a window of max_len + tokens keys or more bounds nothing
   const int64_t win = std::min<int64_t>(window, 0x7FFFFFFF);
   AttnArgs a{(const uint16_t*)q, q_sb, q_st, q_sh, (int)batch, (int)tokens, (int)n_heads, (int)n_kv_heads, (int)G,
-             (int)max_len, (int)rows, cut.tiles, cut.splits, (int)win, scale, k_codes, (const uint32_t*)k_scales,
+             (int)max_len, (int)rows, cut.tiles, cut.splits, (int)win, scale, G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0u, k_codes, (const uint32_t*)k_scales,
              v_codes, (const uint32_t*)v_scales, pos, start, (uint16_t*)out, (float*)workspace};
   const hipStream_t st = (hipStream_t)stream;
   const bool bf = type == BF16X_BF16;
-  const int64_t out_rows = batch * n_kv_heads * rows;
-  if (head_dim == 128) bf ? launch<128, true>(a, cut.rows, blocks, out_rows, st) : launch<128, false>(a, cut.rows, blocks, out_rows, st);
-  else bf ? launch<64, true>(a, cut.rows, blocks, out_rows, st) : launch<64, false>(a, cut.rows, blocks, out_rows, st);
+  if (head_dim == 128) bf ? launch<128, true>(a, cut.rows, st) : launch<128, false>(a, cut.rows, st);
+  else bf ? launch<64, true>(a, cut.rows, st) : launch<64, false>(a, cut.rows, st);
   return launch_status();
 }
