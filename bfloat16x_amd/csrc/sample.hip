@@ -5,23 +5,20 @@
 // logit, then lower index), so the kept set is one threshold in that order: of
 // the 64-bit number (the logit's bits in ascending order, then the complement of
 // the index), which is different for every token.  It is found without sorting
-// the row: the weights of a row span 32 nepers at most (smaller ones round to
-// nothing in 2^-44), which are cut into kBins bins; counts and masses per bin
-// tell the bin (for top-p behind top-k, the few bins) that holds the threshold,
-// and only the tokens of those are sorted.  The steps, one launch each, chunks
-// of a row in parallel:
-//   1. largest and smallest logit of every chunk;
-//   2. count and mass of the bins (rows with top-k or top-p), or the mass of
-//      every chunk (rows without);
-//   3. the bins of the threshold; their tokens to a list; the mass of every
-//      chunk in the bins above (rows with top-k or top-p);
-//   4. one workgroup per row: the list sorted, the threshold, the chunk in which
-//      the running mass passes u, the token.
-// Masses are integers of 2^-44 of the largest weight: their sums are the same in
-// any order, so atomics do not change results, and two neighbouring tokens'
-// border moves by 1e-11 of the total at most, where an fp32 sum would move it by
-// the probability of an unlikely token.  The exponential is a Taylor polynomial
-// of degree 11 in fp64 (relative error 1e-14 on half an octave).
+// the row, in two launches that read the row once (and a few parts of it again):
+//   1. a workgroup per chunk of a row: the chunk's largest logit m_c, the sum of
+//      exp((x - m_c) / T), and count and sum of each of kBins bins of a fixed
+//      width below m_c's (a grid of the logits themselves, so that chunks agree);
+//   2. a workgroup per row: the chunks' bins, scaled by exp((m_c - m) / T), from
+//      the top until the bins are known that hold the thresholds; the tokens of
+//      those bins, which are few, from the chunks that have any, sorted; then the
+//      chunk, and in it the token, at which the running sum passes u.
+// Inside a chunk, weights are integers of 2^-44 of the chunk's largest: their sums
+// are the same in any order, so LDS atomics do not change results.  Across
+// chunks, sums are fp64 in a fixed order.  Two neighbouring tokens' border moves
+// by 1e-11 of the total at most, where an fp32 sum would move it by the
+// probability of an unlikely token.  The exponential is a Taylor polynomial of
+// degree 11 in fp64 (relative error 1e-14 on half an octave).
 #include "bf16x_device.h"
 #include "launch_common.h"
 #include "../../include/bf16x_llama.h"
@@ -32,22 +29,18 @@ using namespace bf16x;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
 
-constexpr int kBins = 1024;
-constexpr int kList = 4096;               // tokens of the threshold's bins that step 4 sorts in LDS
+constexpr int kBins = 1024;               // of a chunk; the last one holds everything below the others
+constexpr int kRest = kBins - 1;
+constexpr int kGroup = 16;                // bins of a group, which all chunks cut at the same cells of the grid
+constexpr int kGroups = kBins / kGroup + 1;
+constexpr int kOpen = kBins / kGroup - 1; // groups of a row; the tokens below them are its rest
+constexpr int kList = 4096;               // tokens of the thresholds' bins that are sorted in LDS
+constexpr int kRanked = 256;              // as many are sorted by counting, more bitonically
 constexpr int kMaxChunks = 256;
-constexpr int kT = 256;                   // threads of steps 1 to 3
-constexpr int kDrawT = 1024;              // threads of step 4
+constexpr int kT = 256;                   // threads per chunk
+constexpr int kDrawT = 512;               // threads per row
 constexpr double kSpan = 32.0;            // nepers; exp(-32) < 2^-46
 constexpr int64_t kMaxVocab = (int64_t)1 << 20;
-
-// What steps 3 and 4 know of the bins of a row.
-struct Cut {
-  uint32_t k_bin, p_first, p_last, sure;  // top-k's bin, top-p's bins, bins surely kept (all below `sure`); ~0: none
-  uint32_t before_k;                      // tokens in the bins before top-k's
-  uint32_t in_k;                          // tokens in it
-  u64 mass_k;                             // mass of the bins before top-k's (no top-k: of all)
-  u64 mass_p;                             // mass of the bins before top-p's first
-};
 
 struct SampleArgs {
   const void* logits;
@@ -61,19 +54,19 @@ struct SampleArgs {
   int32_t* state;
   int32_t* history;
   int64_t history_len;
-  float *cmax, *cmin;                     // [rows][chunks]
+  float* cmax;                            // [rows][chunks]
   int32_t* cidx;                          // [rows][chunks] first index of the chunk's maximum
   u64* cmass;                             // [rows][chunks]
-  u64* hmass;                             // [rows][kBins]
-  uint32_t* hcount;                       // [rows][kBins]
-  uint32_t* listed;                       // [rows] tokens put into the list (more than kList: the list is not whole)
-  Cut* cut;                               // [rows]
-  u64* list;                              // [rows][kList]
+  u64* hmass;                             // [rows][chunks][kBins], where the row has a filter
+  uint32_t* hcount;
+  u64* gmass;                             // [rows][chunks][kGroups]
+  uint32_t* gcount;
 };
 
 struct Setting {
   double inv_t;                           // 0 where T is not above 0
-  bool greedy, k_on, p_on;
+  double bins;                            // bins per unit of the logits: 32 a neper, and not under 32
+  bool greedy, k_on, p_on, m_on;
   uint32_t k;
   double p, min_p;
 };
@@ -86,11 +79,13 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int row) {
   Setting s;
   s.greedy = !(t > 0.f);
   s.inv_t = s.greedy ? 0.0 : 1.0 / (double)t;
+  s.bins = 32.0 * (s.inv_t > 1.0 ? s.inv_t : 1.0);
   s.k_on = !s.greedy && k > 0 && k < a.vocab;
   s.k = (uint32_t)k;
   s.p_on = !s.greedy && p < 1.f;
   s.p = p > 0.f ? (double)p : 0.0;
-  s.min_p = fminf(q, 1.f);
+  s.m_on = !s.greedy && q > 2e-14f;        // (less keeps all that can be drawn)
+  s.min_p = s.m_on ? (double)fminf(q, 1.f) : 0.0;
   return s;
 }
 
@@ -180,11 +175,29 @@ __device__ __forceinline__ u64 mass_of(double w) {
 }
 
 template <class T>
+__device__ __forceinline__ T shfl_xor_t(T v, int o) {
+  if constexpr (sizeof(T) == 8) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    return __builtin_bit_cast(T, (u64)(uint32_t)__shfl_xor((int)(b >> 32), o, 64) << 32 |
+                                     (uint32_t)__shfl_xor((int)b, o, 64));
+  } else {
+    return __shfl_xor(v, o, 64);
+  }
+}
+__device__ __forceinline__ u64 wave_total(u64 v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += shfl_xor_t(v, o);
+  return v;
+}
+template <class T>
 __device__ __forceinline__ T shfl_up_t(T v, int o) {
-  if constexpr (sizeof(T) == 8)
-    return (T)((u64)__shfl_up((uint32_t)(v >> 32), o, 64) << 32 | __shfl_up((uint32_t)v, o, 64));
-  else
+  if constexpr (sizeof(T) == 8) {
+    const u64 b = __builtin_bit_cast(u64, v);
+    return __builtin_bit_cast(T, (u64)(uint32_t)__shfl_up((int)(b >> 32), o, 64) << 32 |
+                                     (uint32_t)__shfl_up((int)b, o, 64));
+  } else {
     return __shfl_up(v, o, 64);
+  }
 }
 
 // Inclusive prefix over the NT threads of a workgroup; `red` holds NT / 64 values.
@@ -210,257 +223,130 @@ __device__ __forceinline__ T block_prefix(T v, T* red, T& total) {
   return before + v;
 }
 
-// The row's maximum, minimum (finite or +inf logits) and first index of the maximum, from its chunks'.
-struct Extremes {
-  float mx, mn;
-  int idx;
-};
-template <int NT>
-__device__ __forceinline__ Extremes extremes_of(const SampleArgs& a, int row) {
-  __shared__ float smx[NT / 64], smn[NT / 64];
-  __shared__ int sidx[NT / 64];
-  Extremes e{-INFINITY, INFINITY, 0x7FFFFFFF};
-  for (int i = threadIdx.x; i < a.chunks; i += NT) {
-    const int64_t at = (int64_t)row * a.chunks + i;
-    const float v = a.cmax[at];
-    const int id = a.cidx[at];
-    if (v > e.mx || (v == e.mx && id < e.idx)) e.mx = v, e.idx = id;
-    e.mn = fminf(e.mn, a.cmin[at]);
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float v = __shfl_xor(e.mx, o, 64);
-    const int id = __shfl_xor(e.idx, o, 64);
-    if (v > e.mx || (v == e.mx && id < e.idx)) e.mx = v, e.idx = id;
-    e.mn = fminf(e.mn, __shfl_xor(e.mn, o, 64));
-  }
-  if ((threadIdx.x & 63) == 0) smx[threadIdx.x >> 6] = e.mx, smn[threadIdx.x >> 6] = e.mn, sidx[threadIdx.x >> 6] = e.idx;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < NT / 64; ++k) {
-    if (smx[k] > e.mx || (smx[k] == e.mx && sidx[k] < e.idx)) e.mx = smx[k], e.idx = sidx[k];
-    e.mn = fminf(e.mn, smn[k]);
-  }
-  return e;
+// Cell of the bins' grid that a logit is in (a whole number; infinite for infinities).
+__device__ __forceinline__ double cell_of(float x, double bins) { return floor((double)x * bins); }
+// Bins that the first group of a grid under `top` lacks.
+__device__ __forceinline__ int lacking(double top) {
+  const double m = top - kGroup * floor(top / kGroup);          // 0 .. 15 (NaN for an infinite top: any cut will do)
+  return m >= 0.0 && m < (double)kGroup ? kGroup - 1 - (int)m : 0;
 }
-// Bins per neper: the row's own span, at most kSpan.
-__device__ __forceinline__ double bins_of(const Extremes& e, double inv_t) {
-  double span = -log_weight(e.mn, e.mx, inv_t);
-  span = span < kSpan ? span : kSpan;
-  return span > 0.0 ? kBins / span : 0.0;
-}
-__device__ __forceinline__ uint32_t bin_of(double y, double bins) { return min((uint32_t)(-y * bins), (uint32_t)kBins - 1); }
-
-template <int TYPE>
-__global__ __launch_bounds__(kT) void sample_max_kernel(SampleArgs a) {
-  __shared__ float smx[kT / 64], smn[kT / 64];
-  __shared__ int sidx[kT / 64];
-  const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x;
-  for (int i = ch * kT + tid; i < kBins; i += a.chunks * kT) {
-    a.hmass[(int64_t)row * kBins + i] = 0;
-    a.hcount[(int64_t)row * kBins + i] = 0;
-  }
-  if (ch == 0 && tid == 0) a.listed[row] = 0;
-  bool vec;
-  const void* p = row_of<TYPE>(a, row, vec);
-  float mx = -INFINITY, mn = INFINITY;
-  int idx = 0x7FFFFFFF;
-  const int end = min(a.vocab, (ch + 1) * a.chunk);
-  for (int i = ch * a.chunk + 8 * tid; i < end; i += 8 * kT) {
-    float x[8];
-    logits8<TYPE>(a, p, vec, i, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (x[e] > mx) mx = x[e], idx = i + e;
-      if (x[e] > -INFINITY) mn = fminf(mn, x[e]);
-    }
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float v = __shfl_xor(mx, o, 64);
-    const int id = __shfl_xor(idx, o, 64);
-    if (v > mx || (v == mx && id < idx)) mx = v, idx = id;
-    mn = fminf(mn, __shfl_xor(mn, o, 64));
-  }
-  if ((tid & 63) == 0) smx[tid >> 6] = mx, smn[tid >> 6] = mn, sidx[tid >> 6] = idx;
-  __syncthreads();
-  if (tid == 0) {
-#pragma unroll
-    for (int k = 1; k < kT / 64; ++k) {
-      if (smx[k] > mx || (smx[k] == mx && sidx[k] < idx)) mx = smx[k], idx = sidx[k];
-      mn = fminf(mn, smn[k]);
-    }
-    const int64_t at = (int64_t)row * a.chunks + ch;
-    a.cmax[at] = mx;
-    a.cmin[at] = mn;
-    a.cidx[at] = idx;
-  }
+// Bin of a logit under a top cell: 0 .. kRest.
+__device__ __forceinline__ int bin_of(float x, double top, double bins) {
+  const double d = top - cell_of(x, bins);
+  return d < (double)kRest ? (int)d : (d >= (double)kRest ? kRest : 0);         // (inf - inf: the top itself)
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kT) void sample_mass_kernel(SampleArgs a) {
+__device__ __forceinline__ void first_max(float& v, int& i, float v2, int i2) {
+  if (v2 > v || (v2 == v && i2 < i)) v = v2, i = i2;
+}
+
+template <int TYPE, int NV>
+__global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
   __shared__ u64 hm[kBins];
   __shared__ uint32_t hc[kBins];
-  __shared__ u64 red[kT / 64];
-  const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x;
-  const Setting s = setting_of(a, row);
-  if (s.greedy) return;
-  const bool bins_on = s.k_on || s.p_on;
-  const Extremes ex = extremes_of<kT>(a, row);
-  const double bins = bins_of(ex, s.inv_t);
-  if (bins_on) {
-    for (int i = tid; i < kBins; i += kT) hm[i] = 0, hc[i] = 0;
-    __syncthreads();
-  }
-  bool vec;
-  const void* p = row_of<TYPE>(a, row, vec);
-  const int end = min(a.vocab, (ch + 1) * a.chunk);
-  u64 sum = 0;
-  for (int i = ch * a.chunk + 8 * tid; i < end; i += 8 * kT) {
-    float x[8];
-    logits8<TYPE>(a, p, vec, i, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double y = log_weight(x[e], ex.mx, s.inv_t);
-      if (x[e] > -INFINITY && y >= -kSpan) {
-        const double w = weight_of(y);
-        if (bins_on) {
-          const uint32_t b = bin_of(y, bins);
-          atomicAdd(&hm[b], mass_of(w));
-          atomicAdd(&hc[b], 1u);
-        } else if (w >= s.min_p) {
-          sum += mass_of(w);
-        }
-      }
-    }
-  }
-  if (!bins_on) {
-    u64 total;
-    block_prefix<kT>(sum, red, total);
-    if (tid == 0) a.cmass[(int64_t)row * a.chunks + ch] = total;
-    return;
-  }
-  __syncthreads();
-  for (int i = tid; i < kBins; i += kT)
-    if (hc[i]) {
-      atomicAdd(&a.hmass[(int64_t)row * kBins + i], hm[i]);
-      atomicAdd(&a.hcount[(int64_t)row * kBins + i], hc[i]);
-    }
-}
-
-// The mass that top-p asks of a kept mass M.
-__device__ __forceinline__ u64 wanted(double p, u64 M) {
-  const u64 t = (u64)ceil(p * (double)M);
-  return t < 1 ? 1 : t > M ? M : t;
-}
-
-template <int TYPE>
-__global__ __launch_bounds__(kT) void sample_list_kernel(SampleArgs a) {
-  constexpr int E = kBins / kT;
-  __shared__ u64 red[kT / 64];
+  static_assert(kT == 256, "");
+  __shared__ u64 red[2][kT / 64];
   __shared__ uint32_t red32[kT / 64];
-  __shared__ Cut cut;
+  __shared__ float smx[kT / 64];
+  __shared__ int sidx[kT / 64];
   const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x;
-  const Setting s = setting_of(a, row);
-  if (!s.k_on && !s.p_on) return;          // (greedy rows have neither)
-  const Extremes ex = extremes_of<kT>(a, row);
-  const double bins = bins_of(ex, s.inv_t);
-  // the bins of the threshold
-  u64 m[E], mass = 0, all_mass;
-  uint32_t c[E], count = 0, all_count;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    m[e] = a.hmass[(int64_t)row * kBins + tid * E + e];
-    c[e] = a.hcount[(int64_t)row * kBins + tid * E + e];
-    mass += m[e];
-    count += c[e];
-  }
-  const u64 m_before = block_prefix<kT>(mass, red, all_mass) - mass;
-  const uint32_t c_before = block_prefix<kT>(count, red32, all_count) - count;
-  if (tid == 0) cut = Cut{~0u, ~0u, ~0u, ~0u, 0, 0, all_mass, 0};
-  __syncthreads();
-  const bool k_cut = s.k_on && s.k < all_count;
-  if (k_cut) {
-    u64 mb = m_before;
-    uint32_t cb = c_before;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (cb < s.k && s.k <= cb + c[e]) cut.k_bin = tid * E + e, cut.before_k = cb, cut.in_k = c[e], cut.mass_k = mb;
-      mb += m[e];
-      cb += c[e];
-    }
-  }
-  __syncthreads();
-  if (s.p_on) {
-    const u64 least = wanted(s.p, cut.mass_k);
-    u64 most_mass = cut.mass_k;
-    if (k_cut) most_mass += a.hmass[(int64_t)row * kBins + cut.k_bin];
-    const u64 most = wanted(s.p, most_mass);
-    u64 mb = m_before;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (mb < least && least <= mb + m[e]) cut.p_first = tid * E + e, cut.mass_p = mb;
-      if (mb < most && most <= mb + m[e]) cut.p_last = tid * E + e;
-      mb += m[e];
-    }
-  }
-  __syncthreads();
-  if (tid == 0) {
-    cut.sure = s.p_on ? cut.p_first : cut.k_bin;
-    if (ch == 0) a.cut[row] = cut;
-  }
-  __syncthreads();
-  const uint32_t sure = s.p_on ? cut.p_first : cut.k_bin;
-  // their tokens, and the mass above them
   bool vec;
   const void* p = row_of<TYPE>(a, row, vec);
-  const int end = min(a.vocab, (ch + 1) * a.chunk);
-  u64 sum = 0;
-  for (int i = ch * a.chunk + 8 * tid; i < end; i += 8 * kT) {
-    float x[8];
-    logits8<TYPE>(a, p, vec, i, x);
+  float x[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) logits8<TYPE>(a, p, vec, ch * (8 * NV * kT) + 8 * (v * kT + tid), x[v]);
+  const Setting s = setting_of(a, row);
+  const bool bins_on = s.k_on || s.p_on || s.m_on;
+  if (bins_on)
+    for (int i = tid; i < kBins; i += kT) hm[i] = 0, hc[i] = 0;
+  float mx = -INFINITY;
+  int idx = 0x7FFFFFFF;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (x[v][e] > mx) mx = x[v][e], idx = ch * (8 * NV * kT) + 8 * (v * kT + tid) + e;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) first_max(mx, idx, __shfl_xor(mx, o, 64), __shfl_xor(idx, o, 64));
+  if ((tid & 63) == 0) smx[tid >> 6] = mx, sidx[tid >> 6] = idx;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kT / 64; ++k) first_max(mx, idx, smx[k], sidx[k]);
+  const int64_t at = (int64_t)row * a.chunks + ch;
+  if (tid == 0) {
+    a.cmax[at] = mx;
+    a.cidx[at] = idx;
+  }
+  if (s.greedy) return;
+  const double top = cell_of(mx, s.bins);
+  u64 sum = 0, rest = 0;
+  uint32_t rest_count = 0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const double y = log_weight(x[e], ex.mx, s.inv_t);
-      if (!(x[e] > -INFINITY && y >= -kSpan)) continue;
-      const uint32_t b = bin_of(y, bins);
-      if (b < sure) {
-        const double w = weight_of(y);
-        if (w >= s.min_p) sum += mass_of(w);
-      } else if ((b >= cut.p_first && b <= cut.p_last && s.p_on) || b == cut.k_bin) {
-        const uint32_t at = atomicAdd(&a.listed[row], 1u);
-        if (at < kList) a.list[(int64_t)row * kList + at] = place_of(x[e], i + e);
+      if (!(x[v][e] > -INFINITY)) continue;
+      const double y = log_weight(x[v][e], mx, s.inv_t);
+      const u64 m = y >= -kSpan ? mass_of(weight_of(y)) : 0;
+      sum += m;
+      if (!bins_on) continue;
+      const int b = bin_of(x[v][e], top, s.bins);
+      if (b == kRest) {                   // (often most of the row: not one address for all)
+        rest += m;
+        ++rest_count;
+      } else {
+        atomicAdd(&hm[b], m);
+        atomicAdd(&hc[b], 1u);
       }
     }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    sum += shfl_xor_t(sum, o);
+    if (bins_on) {
+      rest += shfl_xor_t(rest, o);
+      rest_count += (uint32_t)__shfl_xor((int)rest_count, o, 64);
+    }
   }
-  u64 total;
-  block_prefix<kT>(sum, red, total);
-  if (tid == 0) a.cmass[(int64_t)row * a.chunks + ch] = total;
-}
-
-__device__ __forceinline__ double weight_at(u64 place, const Extremes& ex, double inv_t) {
-  const double y = log_weight(unordered((uint32_t)(place >> 32)), ex.mx, inv_t);
-  return y >= -kSpan ? weight_of(y) : 0.0;
+  if ((tid & 63) == 0) red[0][tid >> 6] = sum, red[1][tid >> 6] = rest, red32[tid >> 6] = rest_count;
+  __syncthreads();                         // (and the atomics are done)
+  if (tid == 0) a.cmass[at] = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
+  if (!bins_on) return;
+#pragma unroll
+  for (int k = 0; k < kBins / kT; ++k) {
+    const int i = k * kT + tid;
+    a.hmass[at * kBins + i] = i == kRest ? (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]) : hm[i];
+    a.hcount[at * kBins + i] = i == kRest ? (red32[0] + red32[1]) + (red32[2] + red32[3]) : hc[i];
+  }
+  if (tid < kGroups) {
+    const int first = tid * kGroup - lacking(top);
+    u64 m = 0;
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      const int b = first + k;
+      if (b >= 0 && b < kRest) m += hm[b], n += hc[b];
+    }
+    a.gmass[at * kGroups + tid] = m;
+    a.gcount[at * kGroups + tid] = n;
+  }
 }
 
 // Threshold of a row whose list is not whole (many tokens of one value): built
 // bit by bit, a pass over the row each, first for top-k, then for top-p.
 template <int TYPE>
-__device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, const Extremes& ex, const void* p, bool vec,
-                                   bool k_cut, u64* red) {
+__device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, float mx, const void* p, bool vec, u64* red) {
   auto above = [&](u64 thr, u64& mass) {
     u64 n = 0, m = 0, total;
     for (int i = 8 * (int)threadIdx.x; i < a.vocab; i += 8 * kDrawT) {
       float x[8];
       logits8<TYPE>(a, p, vec, i, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double y = log_weight(x[e], ex.mx, s.inv_t);
-        if (x[e] > -INFINITY && y >= -kSpan && place_of(x[e], i + e) >= thr) {
+      for (int e = 0; e < 8; ++e)
+        if (x[e] > -INFINITY && place_of(x[e], i + e) >= thr) {
+          const double y = log_weight(x[e], mx, s.inv_t);
           ++n;
-          m += mass_of(weight_of(y));
+          m += y >= -kSpan ? mass_of(weight_of(y)) : 0;
         }
-      }
     }
     block_prefix<kDrawT>(m, red, mass);
     block_prefix<kDrawT>(n, red, total);
@@ -469,14 +355,15 @@ __device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, const 
   // (bits 20 .. 31, the upper ones of an index's complement, are set in every place)
   constexpr u64 kSet = 0xFFF00000ull;
   u64 thr = kSet, M;
-  if (k_cut)
+  if (s.k_on)
     for (int bit = 63; bit >= 0; bit = bit == 32 ? 19 : bit - 1) {
       const u64 t = thr | 1ull << bit;
       if (above(t, M) >= s.k) thr = t;
     }
   if (s.p_on) {
     above(thr, M);
-    const u64 want = wanted(s.p, M);
+    const double least = ceil(s.p * (double)M);
+    const u64 want = least >= 1.0 ? (u64)least : 1;
     u64 pt = kSet;
     for (int bit = 63; bit >= 0; bit = bit == 32 ? 19 : bit - 1) {
       const u64 t = pt | 1ull << bit;
@@ -491,18 +378,29 @@ __device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, const 
 template <int TYPE>
 __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
   __shared__ u64 place[kList];
-  __shared__ u64 prefix[kList];
-  __shared__ u64 cm[kMaxChunks];
+  __shared__ double prefix[kList];         // mass up to a listed token (before that, partial sums)
+  __shared__ uint32_t counts[kDrawT];
+  __shared__ double group_mass[64], bin_mass[kGroup];           // up to a group of bins, up to a bin of the open one
+  __shared__ uint32_t group_count[64], bin_count[kGroup];
+  __shared__ double scale[kMaxChunks];     // exp((m_c - m) / T)
+  __shared__ u64 kept[kMaxChunks];         // kept mass of a chunk, in units of its own
+  __shared__ float cmx[kMaxChunks];
+  __shared__ int below[kMaxChunks];        // bins by which a chunk's top is below the row's, and groups
+  __shared__ int below_group[kMaxChunks];
+  __shared__ uint16_t scan[kMaxChunks];    // chunks that have tokens in the thresholds' bins
+  __shared__ double redd[kDrawT / 64];
   __shared__ u64 red[kDrawT / 64];
-  __shared__ uint32_t first;
-  __shared__ uint32_t in_chunk;
-  __shared__ u64 before_chunk;
-  const int row = blockIdx.x, tid = threadIdx.x;
+  __shared__ float smx[kDrawT / 64];
+  __shared__ int sidx[kDrawT / 64];
+  __shared__ uint32_t listed, in_k, scans, first;
+  __shared__ int in_chunk;
+  __shared__ double before_chunk;
+  constexpr int E = kList / kDrawT;
+  const int row = blockIdx.x, tid = threadIdx.x, C = a.chunks;
+  const int64_t at = (int64_t)row * C;
   const Setting s = setting_of(a, row);
-  const Extremes ex = extremes_of<kDrawT>(a, row);
   const int32_t step = a.state ? a.state[1] : 0;
-  const int64_t u_at = a.state ? (step < 0 ? 0 : step >= a.n_u ? a.n_u - 1 : step) : row;
-  __syncthreads();                         // every thread has read the state that the one that finds the token writes
+  const float uf = a.u[a.state ? (step < 0 ? 0 : step >= a.n_u ? a.n_u - 1 : (int64_t)step) : (int64_t)row];
   auto finish = [&](int64_t token, double logp) {
     a.token[row] = token;
     if (a.logprob) a.logprob[row] = (float)logp;
@@ -512,111 +410,398 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
       a.state[1] = step + 1;
     }
   };
-  if (ex.mx == -INFINITY || s.greedy) {
-    if (tid == 0) ex.mx == -INFINITY ? finish(-1, -INFINITY) : finish(ex.idx, 0.0);
+  // the row's maximum
+  const float cm = tid < C ? a.cmax[at + tid] : -INFINITY;
+  const u64 cmass = tid < C && !s.greedy ? a.cmass[at + tid] : 0;
+  float mx = cm;
+  int idx = tid < C ? a.cidx[at + tid] : 0x7FFFFFFF;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) first_max(mx, idx, __shfl_xor(mx, o, 64), __shfl_xor(idx, o, 64));
+  if ((tid & 63) == 0) smx[tid >> 6] = mx, sidx[tid >> 6] = idx;
+  if (tid == 0) listed = in_k = scans = 0, in_chunk = -1;
+  __syncthreads();                         // (every thread has read the state that the one that finds the token writes)
+#pragma unroll
+  for (int k = 0; k < kDrawT / 64; ++k) first_max(mx, idx, smx[k], sidx[k]);
+  if (mx == -INFINITY || s.greedy) {
+    if (tid == 0) mx == -INFINITY ? finish(-1, -INFINITY) : finish(idx, 0.0);
     return;
   }
   bool vec;
   const void* p = row_of<TYPE>(a, row, vec);
-  const bool filtered = s.k_on || s.p_on;
+  const double top = cell_of(mx, s.bins);
+  double share = 0.0;
+  if (tid < C) {
+    const double y = cm > -INFINITY ? log_weight(cm, mx, s.inv_t) : -INFINITY;
+    const double f = y > -700.0 ? exp(y) : 0.0;
+    share = (double)cmass * f;
+    scale[tid] = f;
+    const int b = cm > -INFINITY ? bin_of(cm, top, s.bins) : kBins;
+    below[tid] = b;
+    below_group[tid] = b < kRest ? (b + lacking(top)) / kGroup : kGroups;
+    cmx[tid] = cm;
+    kept[tid] = cmass;
+  }
+  double total;
+  block_prefix<kDrawT>(share, redd, total);
+  // mass of a token in units of its chunk's maximum, and its weight
+  auto own_mass = [&](float x, float m_c) {
+    const double y = log_weight(x, m_c, s.inv_t);
+    return y >= -kSpan ? mass_of(weight_of(y)) : 0;
+  };
+  auto passes_min = [&](float x) {
+    if (!s.m_on) return true;
+    const double y = log_weight(x, mx, s.inv_t);
+    return y >= -kSpan && weight_of(y) >= s.min_p;
+  };
+
+  const bool ordered_cut = s.k_on || s.p_on;
   u64 thr = 0;
-  for (int i = tid; i < a.chunks; i += kDrawT) cm[i] = a.cmass[(int64_t)row * a.chunks + i];
-  if (filtered) {
-    const Cut cut = a.cut[row];
-    const bool k_cut = cut.k_bin != ~0u;
-    const uint32_t n = a.listed[row];
-    if (n > kList) {
-      thr = threshold_by_passes<TYPE>(a, s, ex, p, vec, k_cut, red);
-      for (int i = tid; i < a.chunks; i += kDrawT) cm[i] = 0;
+  if (ordered_cut || s.m_on) {
+    // bins whose tokens decide: r_first .. r_last and kb (none: -1); rest: the first bin of the row's rest
+    const int off = lacking(top), rest = kOpen * kGroup - off;
+    int r_first = rest + 1, r_last = -1, kb = -1;
+    double mass_k = total, mass_first = 0.0;                    // mass before top-k's bin (all of it), and before r_first
+    uint32_t before_k = 0;
+    if (ordered_cut) {
+      // masses and counts of the groups, chunks in 8 parts, then up to each group
+      {
+        const int K = tid & 63, part = tid >> 6;
+        double m = 0.0;
+        uint32_t n = 0;
+#pragma unroll 4
+        for (int c = part; c < C; c += kDrawT / 64) {
+          const int k = K - below_group[c];
+          const int64_t j = (at + c) * kGroups + max(k, 0);
+          const u64 gm = a.gmass[j];       // (written for every chunk, also one without a token)
+          const uint32_t gc = a.gcount[j];
+          m += k >= 0 ? (double)gm * scale[c] : 0.0;
+          n += k >= 0 ? gc : 0;
+        }
+        prefix[part * 64 + K] = m;
+        counts[part * 64 + K] = n;
+      }
       __syncthreads();
+      if (tid < 64) {
+        double m = 0.0;
+        uint32_t n = 0;
+#pragma unroll
+        for (int k = 0; k < kDrawT / 64; ++k) m += prefix[k * 64 + tid], n += counts[k * 64 + tid];
+        if (tid >= kOpen) m = 0.0, n = 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const double um = shfl_up_t(m, o);
+          const uint32_t un = shfl_up_t(n, o);
+          if (tid >= o) m += um, n += un;
+        }
+        group_mass[tid] = m;
+        group_count[tid] = n;
+      }
+      __syncthreads();
+      // masses and counts up to each bin of group K (bins K kGroup - off + f)
+      int opened = -1;
+      auto open_group = [&](int K) {
+        if (K == opened) return;
+        opened = K;
+        const int f = tid & (kGroup - 1), g = K * kGroup - off + f, lane = tid & 63;
+        double m = 0.0;
+        uint32_t n = 0;
+        for (int c = tid / kGroup; c < C; c += kDrawT / kGroup) {
+          const int b = g - below[c];
+          const int64_t j = (at + c) * kBins + max(b, 0);
+          const u64 hm = a.hmass[j];
+          const uint32_t hc = a.hcount[j];
+          m += b >= 0 ? (double)hm * scale[c] : 0.0;
+          n += b >= 0 ? hc : 0;
+        }
+#pragma unroll
+        for (int o = kGroup; o < 64; o <<= 1) {
+          m += shfl_xor_t(m, o);
+          n += shfl_xor_t(n, o);
+        }
+        __syncthreads();
+        if (lane < kGroup) prefix[(tid >> 6) * kGroup + f] = m, counts[(tid >> 6) * kGroup + f] = n;
+        __syncthreads();
+        if (tid < kGroup) {
+          m = 0.0;
+          n = 0;
+#pragma unroll
+          for (int k = 0; k < kDrawT / 64; ++k) m += prefix[k * kGroup + tid], n += counts[k * kGroup + tid];
+#pragma unroll
+          for (int o = 1; o < kGroup; o <<= 1) {
+            const double um = shfl_up_t(m, o);
+            const uint32_t un = shfl_up_t(n, o);
+            if (tid >= o) m += um, n += un;
+          }
+          bin_mass[tid] = m + (K ? group_mass[K - 1] : 0.0);
+          bin_count[tid] = n + (K ? group_count[K - 1] : 0);
+        }
+        __syncthreads();
+      };
+      const int lane = tid & 63;
+      auto first_of = [](bool ok) {        // lowest lane with it, -1 for none
+        const u64 all = __ballot(ok);
+        return all ? (int)__builtin_ctzll(all) : -1;
+      };
+      // the bin in which the mass reaches `want`, and the mass before it
+      auto bin_at = [&](double want, double& before) {
+        const int K = first_of(lane < kOpen && group_mass[lane] >= want);
+        if (K < 0) {
+          before = group_mass[kOpen - 1];
+          return rest;
+        }
+        open_group(K);
+        int f = first_of(lane < kGroup && bin_mass[lane & (kGroup - 1)] >= want);
+        f = f < 0 ? kGroup - 1 : f;        // (a rounding between the two sums)
+        before = f ? bin_mass[f - 1] : K ? group_mass[K - 1] : 0.0;
+        return max(K * kGroup - off + f, 0);
+      };
+      double most = s.p * total;
+      if (s.k_on) {
+        const int K = first_of(lane < kOpen && group_count[lane] >= s.k);
+        kb = rest;                         // (where not even all groups hold so many)
+        before_k = group_count[kOpen - 1];
+        mass_k = group_mass[kOpen - 1];
+        if (K >= 0) {
+          open_group(K);
+          const int f = first_of(lane < kGroup && bin_count[lane & (kGroup - 1)] >= s.k);
+          kb = K * kGroup - off + f;
+          before_k = f ? bin_count[f - 1] : K ? group_count[K - 1] : 0;
+          mass_k = f ? bin_mass[f - 1] : K ? group_mass[K - 1] : 0.0;
+          most = s.p * bin_mass[f];
+        }
+      }
+      if (s.p_on) {
+        double unused;
+        r_first = bin_at(s.p * mass_k, mass_first);
+        r_last = max(bin_at(most, unused), r_first);
+      } else {
+        r_first = r_last = kb;
+        mass_first = mass_k;
+      }
+    }
+    // the bin of the smallest weight that min-p keeps, and its neighbours: tokens from there on are looked at one by one
+    int sure = r_first;                    // bins below are kept as a whole
+    bool min_only = !ordered_cut;
+    if (s.m_on) {
+      const double least = (double)mx + log(s.min_p) / s.inv_t;
+      const double d = mx == INFINITY ? 0.0 : top - floor(least * s.bins);
+      const int m = d < (double)rest ? (int)(d > 0.0 ? d : 0.0) : rest;
+      const int m_first = max(m - 1, 0), m_last = min(m + 1, rest);
+      sure = min(sure, m_first);
+      if (min_only || m_last < r_first) {
+        min_only = true;
+        r_first = m_last + 1, r_last = m_last, kb = -1;
+      }
+    }
+    const int far = max(r_last, r_first - 1);                   // the last bin to look at, kb apart
+    // a wave per chunk: its mass in the bins below `sure`, and whether it has tokens in those to look at
+    const int Ks = (sure + off) / kGroup;
+    for (int c = tid >> 6; c < C; c += kDrawT / 64) {
+      const int lane = tid & 63, k = lane - below_group[c], b = Ks * kGroup - off + lane - below[c];
+      u64 sum = 0;
+      if (lane < Ks && k >= 0) sum = a.gmass[(at + c) * kGroups + k];
+      if (lane < kGroup && Ks * kGroup - off + lane < sure && b >= 0) sum += a.hmass[(at + c) * kBins + b];
+      bool any = below[c] < kBins && (far >= rest || kb >= rest);
+      for (int j = max(sure - below[c], 0) + lane; j <= far - below[c]; j += 64)
+        any = any || a.hcount[(at + c) * kBins + min(j, kRest)] > 0;
+      if (kb >= below[c] && kb < rest) any = any || a.hcount[(at + c) * kBins + kb - below[c]] > 0;
+      sum = wave_total(sum);
+      if (lane == 0) kept[c] = sum;
+      if (__any(any) && lane == 0) scan[atomicAdd(&scans, 1u)] = (uint16_t)c;
+    }
+    __syncthreads();
+    // their tokens: first by bounds in fp32, a little wide, then by their bins
+    auto bound = [&](int bin, double sign) {
+      const double v = (top - (double)bin) / s.bins;
+      return mx < INFINITY ? (float)(v + sign * (1e-6 * fabs(v) + 0.01 / s.bins)) : (float)sign * INFINITY;
+    };
+    const float lo1 = far >= rest ? -INFINITY : bound(far, -1.0), hi1 = sure > 0 ? bound(sure - 1, 1.0) : INFINITY;
+    const float lo2 = kb < 0 ? INFINITY : kb >= rest ? -INFINITY : bound(kb, -1.0);
+    const float hi2 = kb < 0 ? -INFINITY : kb > 0 ? bound(kb - 1, 1.0) : INFINITY;
+    constexpr int U = 4;                   // reads in flight
+    const int shift = __builtin_ctz(a.chunk / 8), jobs = (int)scans << shift;
+    for (int j0 = tid - (tid & 63); j0 < jobs; j0 += U * kDrawT) {              // (whole waves)
+      float x[U][8];
+      int at_[U];
+#pragma unroll
+      for (int v = 0; v < U; ++v) {
+        const int j = min(j0 + (tid & 63) + v * kDrawT, jobs - 1);
+        at_[v] = scan[j >> shift] * a.chunk + 8 * (j & ((1 << shift) - 1));
+        logits8<TYPE>(a, p, vec, at_[v], x[v]);
+      }
+      uint32_t hits = 0;
+#pragma unroll
+      for (int v = 0; v < U; ++v) {
+        uint32_t h = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = x[v][e];
+          h |= (uint32_t)((((y >= lo1) & (y <= hi1)) | ((y >= lo2) & (y <= hi2))) & (y > -INFINITY)) << e;
+        }
+        hits |= (j0 + (tid & 63) + v * kDrawT < jobs ? h : 0u) << (8 * v);
+      }
+      if (!__any(hits != 0)) continue;
+      uint32_t all, from = wave_prefix(__builtin_popcount(hits), tid & 63, all);
+      uint32_t base = 0;
+      if ((tid & 63) == 0) base = atomicAdd(&listed, all);
+      from += __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+      for (int v = 0; v < U; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (hits >> (8 * v + e) & 1) {
+            if (from < kList) place[from] = place_of(x[v][e], at_[v] + e);
+            ++from;
+          }
+    }
+    __syncthreads();
+    const bool whole = listed <= kList;
+    const int found = whole ? (int)listed : 0;
+    __syncthreads();
+    // what is found by the bounds alone leaves the list again; what only min-p decides is counted at once
+    if (tid == 0 && whole) listed = 0;
+    __syncthreads();
+    uint32_t mine_n = 0, mine_k = 0;
+    for (int i = tid; i < found; i += kDrawT) {
+      const float y = unordered((uint32_t)(place[i] >> 32));
+      const int b = min(bin_of(y, top, s.bins), rest);
+      if ((b >= r_first && b <= r_last) || b == kb) {
+        ++mine_n;
+        mine_k += b == kb;
+      } else {
+        const uint32_t c = ~(uint32_t)place[i] / (uint32_t)a.chunk;
+        if (b >= sure && b < r_first && passes_min(y)) atomicAdd(&kept[c], own_mass(y, cmx[c]));
+        place[i] = 0;
+      }
+    }
+    if (mine_n) atomicAdd(&listed, mine_n);
+    if (mine_k) atomicAdd(&in_k, mine_k);
+    __syncthreads();
+    const uint32_t n = listed;
+    if (!whole && min_only) {              // (a row of almost nothing else: chunk by chunk, no list)
       for (int i = 8 * tid; i < a.vocab; i += 8 * kDrawT) {
         float x[8];
         logits8<TYPE>(a, p, vec, i, x);
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const double y = log_weight(x[e], ex.mx, s.inv_t);
-          if (x[e] > -INFINITY && y >= -kSpan && place_of(x[e], i + e) >= thr) {
-            const double w = weight_of(y);
-            if (w >= s.min_p) sum += mass_of(w);
-          }
+          const int b = min(bin_of(x[e], top, s.bins), rest);
+          if (x[e] > -INFINITY && b >= sure && b < r_first && passes_min(x[e])) sum += own_mass(x[e], cmx[i / a.chunk]);
         }
-        if (sum) atomicAdd(&cm[i / a.chunk], sum);              // (a chunk is a multiple of 8)
+        if (sum) atomicAdd(&kept[i / a.chunk], sum);
+      }
+    } else if (!whole) {
+      thr = threshold_by_passes<TYPE>(a, s, mx, p, vec, red);
+      if (tid < C) kept[tid] = 0;
+      __syncthreads();
+      for (int i = 8 * tid; i < a.vocab; i += 8 * kDrawT) {
+        const int c = i / a.chunk;         // (a chunk is a multiple of 8)
+        float x[8];
+        logits8<TYPE>(a, p, vec, i, x);
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (x[e] > -INFINITY && place_of(x[e], i + e) >= thr && passes_min(x[e])) sum += own_mass(x[e], cmx[c]);
+        if (sum) atomicAdd(&kept[c], sum);
       }
     } else if (n) {
-      // the list in descending order (bitonic), padded with zeros
-      int size = 64;
-      while (size < (int)n) size *= 2;
-      for (int i = tid; i < size; i += kDrawT) place[i] = i < (int)n ? a.list[(int64_t)row * kList + i] : 0;
-      for (int w = 2; w <= size; w *= 2)
-        for (int h = w / 2; h >= 1; h /= 2) {
-          __syncthreads();
-          for (int i = tid; i < size / 2; i += kDrawT) {
-            const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
-            const u64 x = place[lo], y = place[hi];
-            if ((x < y) == ((lo & w) == 0)) place[lo] = y, place[hi] = x;
+      // the list in descending order: by rank, or where it is long bitonic, padded with zeros
+      if (found <= kRanked) {
+        const u64 mine = tid < found ? place[tid] : 0;
+        uint32_t rank = 0;
+        if (tid < found)
+#pragma unroll 16
+          for (int i = 0; i < found; ++i) rank += place[i] > mine;
+        __syncthreads();
+        if (mine) place[rank] = mine;
+      } else {
+        int size = 2 * kRanked;
+        while (size < found) size *= 2;
+        for (int i = found + tid; i < size; i += kDrawT) place[i] = 0;
+        for (int w = 2; w <= size; w *= 2)
+          for (int h = w / 2; h >= 1; h /= 2) {
+            __syncthreads();
+            for (int i = tid; i < size / 2; i += kDrawT) {
+              const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
+              const u64 x = place[lo], y = place[hi];
+              if ((x < y) == ((lo & w) == 0)) place[lo] = y, place[hi] = x;
+            }
           }
-        }
+      }
       __syncthreads();
-      // inclusive masses, 4 consecutive entries per thread
-      u64 m[kList / kDrawT], sum = 0, total;
+      // their masses, then inclusive sums over E consecutive entries per thread
+      auto list_mass = [&](u64 pl) { return own_mass(unordered((uint32_t)(pl >> 32)), cmx[~(uint32_t)pl / (uint32_t)a.chunk]); };
+      for (int i = tid; i < kList; i += kDrawT)
+        prefix[i] = i < (int)n ? (double)list_mass(place[i]) * scale[~(uint32_t)place[i] / (uint32_t)a.chunk] : 0.0;
+      __syncthreads();
+      double m[E], sum = 0.0, all;
 #pragma unroll
-      for (int e = 0; e < kList / kDrawT; ++e) {
-        const int i = tid * (kList / kDrawT) + e;
-        m[e] = i < (int)n ? mass_of(weight_at(place[i], ex, s.inv_t)) : 0;
+      for (int e = 0; e < E; ++e) {
+        m[e] = prefix[tid * E + e];
         sum += m[e];
       }
-      u64 before = block_prefix<kDrawT>(sum, red, total) - sum;
+      double before = block_prefix<kDrawT>(sum, redd, all) - sum;
 #pragma unroll
-      for (int e = 0; e < kList / kDrawT; ++e) {
+      for (int e = 0; e < E; ++e) {
         before += m[e];
-        prefix[tid * (kList / kDrawT) + e] = before;
+        prefix[tid * E + e] = before;
       }
       uint32_t last = n - 1;                                    // the last entry that top-k keeps
-      u64 M = cut.mass_k;
+      double M = total;
       if (tid == 0) first = n;
       __syncthreads();
-      if (k_cut) {                                              // its bin's tokens are the list's last
-        const uint32_t from = n - cut.in_k;
-        last = from + (s.k - cut.before_k) - 1;
-        M += prefix[last] - (from ? prefix[from - 1] : 0);
+      if (s.k_on && s.k - before_k <= in_k) {                   // its bin's tokens are the list's last
+        const uint32_t from = n - in_k;
+        last = from + (s.k - before_k) - 1;
+        M = mass_k + prefix[last] - (from ? prefix[from - 1] : 0.0);
       }
       if (s.p_on) {
-        const u64 want = wanted(s.p, M);
+        const double want = s.p * M;
 #pragma unroll
-        for (int e = 0; e < kList / kDrawT; ++e) {
-          const uint32_t i = tid * (kList / kDrawT) + e;
-          if (i < n && cut.mass_p + prefix[i] >= want && (i == 0 || cut.mass_p + prefix[i - 1] < want)) first = i;
+        for (int e = 0; e < E; ++e) {
+          const uint32_t i = tid * E + e;
+          if (i < n && mass_first + prefix[i] >= want) atomicMin(&first, i);
         }
         __syncthreads();
         last = min(last, first);
       }
       thr = place[last];
-#pragma unroll
-      for (int e = 0; e < kList / kDrawT; ++e) {
-        const uint32_t i = tid * (kList / kDrawT) + e;
-        if (i <= last) {
-          const double w = weight_at(place[i], ex, s.inv_t);
-          if (w >= s.min_p) atomicAdd(&cm[(uint32_t)~(uint32_t)place[i] / (uint32_t)a.chunk], mass_of(w));
-        }
-      }
+      for (int i = tid; i <= (int)last; i += kDrawT)
+        if (passes_min(unordered((uint32_t)(place[i] >> 32))))
+          atomicAdd(&kept[~(uint32_t)place[i] / (uint32_t)a.chunk], list_mass(place[i]));
     }
+    __syncthreads();
+  }
+  // the chunk, then the token, at which the running mass passes u
+  const u64 mine = tid < C ? kept[tid] : 0;
+  const double part = mine ? (double)mine * scale[tid] : 0.0;
+  const double upto = block_prefix<kDrawT>(part, redd, total);
+  const double want = uf > 0.f ? (double)fminf(uf, 1.f) * total : 0.0;
+  if (part > 0.0 && want < upto && want >= upto - part) {
+    in_chunk = tid;
+    before_chunk = upto - part;
   }
   __syncthreads();
-  // the chunk, then the token, at which the running mass passes u
-  u64 total;
-  const u64 mine = tid < a.chunks ? cm[tid] : 0;
-  const u64 upto = block_prefix<kDrawT>(mine, red, total);
-  const float uf = a.u[u_at];
-  u64 want = uf > 0.f ? (u64)((double)fminf(uf, 1.f) * (double)total) : 0;
-  want = want < total ? want : total - 1;
-  if (upto > want && upto - mine <= want) in_chunk = tid, before_chunk = upto - mine;
+  const bool none = in_chunk < 0;
   __syncthreads();
-  const int c0 = (int)in_chunk * a.chunk, end = min(a.vocab, c0 + a.chunk);
-  u64 passed = before_chunk;
+  if (none) {                              // u = 1, or a rounding at a border: the last token before it
+    if (part > 0.0 && want >= upto - part) atomicMax(&in_chunk, tid);
+    __syncthreads();
+    if (tid == in_chunk) before_chunk = upto - part;
+    __syncthreads();
+  }
+  if (in_chunk < 0) {                      // (no kept mass at all: not reached, as the maximum is always kept)
+    if (tid == 0) finish(idx, 0.0);
+    return;
+  }
+  const int ch = in_chunk, c0 = ch * a.chunk, end = min(a.vocab, c0 + a.chunk);
+  const double f = scale[ch], over = (want - before_chunk) / f;
+  u64 aim = over > 0.0 ? (u64)over : 0;
+  aim = aim < kept[ch] ? aim : kept[ch] - 1;
+  u64 passed = 0;
   for (int j0 = c0; j0 < end; j0 += 8 * kDrawT) {
     const int i = j0 + 8 * tid;
-    u64 m[8], sum = 0, part;
+    u64 m[8], sum = 0, all;
 #pragma unroll
     for (int e = 0; e < 8; ++e) m[e] = 0;
     if (i < end) {
@@ -624,24 +809,20 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
       logits8<TYPE>(a, p, vec, i, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const double y = log_weight(x[e], ex.mx, s.inv_t);
-        if (x[e] > -INFINITY && y >= -kSpan && (!filtered || place_of(x[e], i + e) >= thr)) {
-          const double w = weight_of(y);
-          if (w >= s.min_p) m[e] = mass_of(w);
-        }
+        if (x[e] > -INFINITY && place_of(x[e], i + e) >= thr && passes_min(x[e])) m[e] = own_mass(x[e], cmx[ch]);
         sum += m[e];
       }
     }
-    u64 before = passed + block_prefix<kDrawT>(sum, red, part) - sum;
-    if (before <= want && want < before + sum) {
+    u64 before = passed + block_prefix<kDrawT>(sum, red, all) - sum;
+    if (before <= aim && aim < before + sum) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (before <= want && want < before + m[e]) finish(i + e, log((double)m[e] / (double)total));
+        if (before <= aim && aim < before + m[e]) finish(i + e, log((double)m[e] * f / total));
         before += m[e];
       }
     }
-    passed += part;
-    if (passed > want) break;
+    passed += all;
+    if (passed > aim) break;
   }
 }
 
@@ -655,7 +836,7 @@ int64_t chunk_of(int64_t rows) { return rows >= 64 ? 16384 : 4096; }
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Layout {
-  int64_t cmax, cmin, cidx, cmass, hmass, hcount, listed, cut, list, bytes;
+  int64_t cmax, cidx, cmass, hmass, hcount, gmass, gcount, bytes;
 };
 Layout layout_of(int64_t rows, int64_t chunks) {
   Layout l;
@@ -666,24 +847,21 @@ Layout layout_of(int64_t rows, int64_t chunks) {
     return here;
   };
   l.cmax = take(rows * chunks * 4);
-  l.cmin = take(rows * chunks * 4);
   l.cidx = take(rows * chunks * 4);
   l.cmass = take(rows * chunks * 8);
-  l.hmass = take(rows * kBins * 8);
-  l.hcount = take(rows * kBins * 4);
-  l.listed = take(rows * 4);
-  l.cut = take(rows * (int64_t)sizeof(Cut));
-  l.list = take(rows * kList * 8);
+  l.hmass = take(rows * chunks * kBins * 8);
+  l.hcount = take(rows * chunks * kBins * 4);
+  l.gmass = take(rows * chunks * kGroups * 8);
+  l.gcount = take(rows * chunks * kGroups * 4);
   l.bytes = at;
   return l;
 }
 
 template <int TYPE>
-void launch(const SampleArgs& a, int64_t rows, bool any_draw, bool any_filter, hipStream_t st) {
+void launch(const SampleArgs& a, int64_t rows, hipStream_t st) {
   const dim3 grid((unsigned)a.chunks, (unsigned)rows);
-  hipLaunchKernelGGL(sample_max_kernel<TYPE>, grid, dim3(kT), 0, st, a);
-  if (any_draw) hipLaunchKernelGGL(sample_mass_kernel<TYPE>, grid, dim3(kT), 0, st, a);
-  if (any_filter) hipLaunchKernelGGL(sample_list_kernel<TYPE>, grid, dim3(kT), 0, st, a);
+  if (a.chunk == 4096) hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 2>), grid, dim3(kT), 0, st, a);
+  else hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 8>), grid, dim3(kT), 0, st, a);
   hipLaunchKernelGGL(sample_draw_kernel<TYPE>, dim3((unsigned)rows), dim3(kDrawT), 0, st, a);
 }
 
@@ -714,15 +892,11 @@ extern "C" int bf16x_sample(const void* logits, int32_t type, int64_t row_stride
   if (rows == 0) return BF16X_OK;
   char* w = (char*)workspace;
   SampleArgs a{logits, row_stride, (int)vocab, (int)chunk, (int)chunks, u, n_u, *settings, token, logprob, state,
-               history, history_len, (float*)(w + l.cmax), (float*)(w + l.cmin), (int32_t*)(w + l.cidx),
-               (u64*)(w + l.cmass), (u64*)(w + l.hmass), (uint32_t*)(w + l.hcount), (uint32_t*)(w + l.listed),
-               (Cut*)(w + l.cut), (u64*)(w + l.list)};
-  const bf16x_sample_settings& s = *settings;
-  const bool draw = s.temperature || s.temperature_all > 0.f;
-  const bool filter = draw && (s.top_k || s.top_p || (s.top_k_all > 0 && s.top_k_all < vocab) || s.top_p_all < 1.f);
+               history, history_len, (float*)(w + l.cmax), (int32_t*)(w + l.cidx), (u64*)(w + l.cmass),
+               (u64*)(w + l.hmass), (uint32_t*)(w + l.hcount), (u64*)(w + l.gmass), (uint32_t*)(w + l.gcount)};
   const hipStream_t st = (hipStream_t)stream;
-  if (wide) launch<BF16X_F32>(a, rows, draw, filter, st);
-  else if (type == BF16X_F16) launch<BF16X_F16>(a, rows, draw, filter, st);
-  else launch<BF16X_BF16>(a, rows, draw, filter, st);
+  if (wide) launch<BF16X_F32>(a, rows, st);
+  else if (type == BF16X_F16) launch<BF16X_F16>(a, rows, st);
+  else launch<BF16X_BF16>(a, rows, st);
   return launch_status();
 }
