@@ -19,6 +19,8 @@
 // by 1e-11 of the total at most, where an fp32 sum would move it by the
 // probability of an unlikely token.  The exponential is a Taylor polynomial of
 // degree 11 in fp64 (relative error 1e-14 on half an octave).
+#include <cfloat>
+
 #include "bf16x_device.h"
 #include "launch_common.h"
 #include "../../include/bf16x_llama.h"
@@ -35,7 +37,7 @@ constexpr int kGroup = 16;                // bins of a group, which all chunks c
 constexpr int kGroups = kBins / kGroup + 1;
 constexpr int kOpen = kBins / kGroup - 1; // groups of a row; the tokens below them are its rest
 constexpr int kList = 4096;               // tokens of the thresholds' bins that are sorted in LDS
-constexpr int kRanked = 256;              // as many are sorted by counting, more bitonically
+constexpr int kRanked = 512;              // as many are sorted by counting, more bitonically
 constexpr int kMaxChunks = 256;
 constexpr int kT = 256;                   // threads per chunk
 constexpr int kDrawT = 512;               // threads per row
@@ -58,7 +60,7 @@ struct SampleArgs {
   int32_t* cidx;                          // [rows][chunks] first index of the chunk's maximum
   u64* cmass;                             // [rows][chunks]
   u64* hmass;                             // [rows][chunks][kBins], where the row has a filter
-  uint32_t* hcount;
+  uint32_t* hcount;                       // ... where it has top-k
   u64* gmass;                             // [rows][chunks][kGroups]
   uint32_t* gcount;
 };
@@ -89,48 +91,58 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int row) {
   return s;
 }
 
-// Logits i .. i + 7 (i a multiple of 8) as fp32; -inf for NaN and beyond the row.
 template <int TYPE>
-__device__ __forceinline__ void logits8(const SampleArgs& a, const void* row, bool vec, int i, float (&x)[8]) {
-  if (vec && i + 8 <= a.vocab) {
-    if constexpr (TYPE == BF16X_F32) {
-      const f4 p = *(const f4*)((const float*)row + i), q = *(const f4*)((const float*)row + i + 4);
+__device__ __forceinline__ float logit(const void* row, int i) {
+  if constexpr (TYPE == BF16X_F32) return ((const float*)row)[i];
+  else if constexpr (TYPE == BF16X_BF16) return __uint_as_float((uint32_t)((const uint16_t*)row)[i] << 16);
+  else return (float)((const _Float16*)row)[i];
+}
+
+// Groups of 8 logits at i[v] .. i[v] + 7 (multiples of 8) as fp32, -inf beyond
+// the row; NaN stays, and is no token as it is not > -inf.  All N groups are
+// requested at once: vec (the same for all lanes) says that groups are whole and
+// aligned, and the indices are cut to the row rather than branched on.
+template <int TYPE, int N>
+__device__ __forceinline__ void logits8(const SampleArgs& a, const void* row, bool vec, const int (&i)[N],
+                                        float (&x)[N][8]) {
+  if (vec) {
+    u32x4 r[N][TYPE == BF16X_F32 ? 2 : 1];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = p[e], x[4 + e] = q[e];
-    } else {
-      const u32x4 r = *(const u32x4*)((const uint16_t*)row + i);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (TYPE == BF16X_BF16) {
-          x[2 * e] = bf16lo_to_f32(w[e]);
-          x[2 * e + 1] = bf16hi_to_f32(w[e]);
-        } else {
-          x[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-          x[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
-        }
-      }
+    for (int v = 0; v < N; ++v) {
+      const int j = min(i[v], a.vocab - 8);
+      const u32x4* q = (const u32x4*)((const char*)row + (int64_t)j * (TYPE == BF16X_F32 ? 4 : 2));
+      r[v][0] = q[0];
+      if constexpr (TYPE == BF16X_F32) r[v][1] = q[1];
     }
+#pragma unroll
+    for (int v = 0; v < N; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float y;
+        if constexpr (TYPE == BF16X_F32) {
+          y = __uint_as_float(r[v][e >> 2][e & 3]);
+        } else {
+          const uint32_t w = r[v][0][e >> 1];
+          if constexpr (TYPE == BF16X_BF16) y = e & 1 ? bf16hi_to_f32(w) : bf16lo_to_f32(w);
+          else y = (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? w >> 16 : w));
+        }
+        x[v][e] = i[v] < a.vocab ? y : -INFINITY;
+      }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float v = -INFINITY;
-      if (i + e < a.vocab) {
-        if constexpr (TYPE == BF16X_F32) v = ((const float*)row)[i + e];
-        else if constexpr (TYPE == BF16X_BF16) v = __uint_as_float((uint32_t)((const uint16_t*)row)[i + e] << 16);
-        else v = (float)((const _Float16*)row)[i + e];
-      }
-      x[e] = v;
-    }
-  }
+    for (int v = 0; v < N; ++v)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
+      for (int e = 0; e < 8; ++e) {
+        const float y = logit<TYPE>(row, min(i[v] + e, a.vocab - 1));
+        x[v][e] = i[v] + e < a.vocab ? y : -INFINITY;
+      }
+  }
 }
 
 template <int TYPE>
 __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row, bool& vec) {
   const char* p = (const char*)a.logits + (int64_t)row * a.stride * (TYPE == BF16X_F32 ? 4 : 2);
-  vec = ((uintptr_t)p & 15u) == 0;
+  vec = ((uintptr_t)p & 15u) == 0 && a.vocab % 8 == 0;
   return p;
 }
 
@@ -253,8 +265,10 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
   bool vec;
   const void* p = row_of<TYPE>(a, row, vec);
   float x[NV][8];
+  int at_[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) logits8<TYPE>(a, p, vec, ch * (8 * NV * kT) + 8 * (v * kT + tid), x[v]);
+  for (int v = 0; v < NV; ++v) at_[v] = ch * (8 * NV * kT) + 8 * (v * kT + tid);
+  logits8<TYPE>(a, p, vec, at_, x);
   const Setting s = setting_of(a, row);
   const bool bins_on = s.k_on || s.p_on || s.m_on;
   if (bins_on)
@@ -265,7 +279,7 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (x[v][e] > mx) mx = x[v][e], idx = ch * (8 * NV * kT) + 8 * (v * kT + tid) + e;
+      if (x[v][e] > mx) mx = x[v][e], idx = at_[v] + e;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) first_max(mx, idx, __shfl_xor(mx, o, 64), __shfl_xor(idx, o, 64));
   if ((tid & 63) == 0) smx[tid >> 6] = mx, sidx[tid >> 6] = idx;
@@ -296,7 +310,7 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
         ++rest_count;
       } else {
         atomicAdd(&hm[b], m);
-        atomicAdd(&hc[b], 1u);
+        if (s.k_on) atomicAdd(&hc[b], 1u);
       }
     }
 #pragma unroll
@@ -315,7 +329,7 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
   for (int k = 0; k < kBins / kT; ++k) {
     const int i = k * kT + tid;
     a.hmass[at * kBins + i] = i == kRest ? (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]) : hm[i];
-    a.hcount[at * kBins + i] = i == kRest ? (red32[0] + red32[1]) + (red32[2] + red32[3]) : hc[i];
+    if (s.k_on) a.hcount[at * kBins + i] = i == kRest ? (red32[0] + red32[1]) + (red32[2] + red32[3]) : hc[i];
   }
   if (tid < kGroups) {
     const int first = tid * kGroup - lacking(top);
@@ -327,7 +341,7 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
       if (b >= 0 && b < kRest) m += hm[b], n += hc[b];
     }
     a.gmass[at * kGroups + tid] = m;
-    a.gcount[at * kGroups + tid] = n;
+    if (s.k_on) a.gcount[at * kGroups + tid] = n;
   }
 }
 
@@ -338,8 +352,8 @@ __device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, float 
   auto above = [&](u64 thr, u64& mass) {
     u64 n = 0, m = 0, total;
     for (int i = 8 * (int)threadIdx.x; i < a.vocab; i += 8 * kDrawT) {
-      float x[8];
-      logits8<TYPE>(a, p, vec, i, x);
+      float x1[1][8], (&x)[8] = x1[0];
+      logits8<TYPE>(a, p, vec, {i}, x1);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (x[e] > -INFINITY && place_of(x[e], i + e) >= thr) {
@@ -473,7 +487,7 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
           const int k = K - below_group[c];
           const int64_t j = (at + c) * kGroups + max(k, 0);
           const u64 gm = a.gmass[j];       // (written for every chunk, also one without a token)
-          const uint32_t gc = a.gcount[j];
+          const uint32_t gc = s.k_on ? a.gcount[j] : 0;
           m += k >= 0 ? (double)gm * scale[c] : 0.0;
           n += k >= 0 ? gc : 0;
         }
@@ -509,7 +523,7 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
           const int b = g - below[c];
           const int64_t j = (at + c) * kBins + max(b, 0);
           const u64 hm = a.hmass[j];
-          const uint32_t hc = a.hcount[j];
+          const uint32_t hc = s.k_on ? a.hcount[j] : 0;
           m += b >= 0 ? (double)hm * scale[c] : 0.0;
           n += b >= 0 ? hc : 0;
         }
@@ -596,30 +610,53 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
     const int far = max(r_last, r_first - 1);                   // the last bin to look at, kb apart
     // a wave per chunk: its mass in the bins below `sure`, and whether it has tokens in those to look at
     const int Ks = (sure + off) / kGroup;
-    for (int c = tid >> 6; c < C; c += kDrawT / 64) {
-      const int lane = tid & 63, k = lane - below_group[c], b = Ks * kGroup - off + lane - below[c];
-      u64 sum = 0;
-      if (lane < Ks && k >= 0) sum = a.gmass[(at + c) * kGroups + k];
-      if (lane < kGroup && Ks * kGroup - off + lane < sure && b >= 0) sum += a.hmass[(at + c) * kBins + b];
-      bool any = below[c] < kBins && (far >= rest || kb >= rest);
-      for (int j = max(sure - below[c], 0) + lane; j <= far - below[c]; j += 64)
-        any = any || a.hcount[(at + c) * kBins + min(j, kRest)] > 0;
-      if (kb >= below[c] && kb < rest) any = any || a.hcount[(at + c) * kBins + kb - below[c]] > 0;
-      sum = wave_total(sum);
-      if (lane == 0) kept[c] = sum;
-      if (__any(any) && lane == 0) scan[atomicAdd(&scans, 1u)] = (uint16_t)c;
+    // (counts are there for top-k alone; for the others only tokens of some mass matter)
+    auto tokens_in = [&](int64_t j) -> uint32_t { return s.k_on ? a.hcount[j] : a.hmass[j] != 0; };
+    constexpr int B = 4;                   // chunks of a wave at once
+    for (int c0 = tid >> 6; c0 < C; c0 += B * (kDrawT / 64)) {
+      const int lane = tid & 63;
+      u64 sum[B];
+      uint32_t any[B];
+#pragma unroll
+      for (int v = 0; v < B; ++v) {
+        const int c = min(c0 + v * (kDrawT / 64), C - 1);
+        const int k = lane - below_group[c], bf = Ks * kGroup - off + lane, b = bf - below[c];
+        const int j = max(sure - below[c], 0) + lane;
+        const u64 g = lane < Ks && k >= 0 ? a.gmass[(at + c) * kGroups + k] : 0;
+        const u64 h = lane < kGroup && bf < sure && b >= 0 ? a.hmass[(at + c) * kBins + b] : 0;
+        any[v] = j <= far - below[c] ? tokens_in((at + c) * kBins + min(j, kRest)) : 0;
+        if (kb >= below[c] && kb < rest) any[v] |= a.hcount[(at + c) * kBins + kb - below[c]];
+        sum[v] = g + h;
+      }
+#pragma unroll
+      for (int v = 0; v < B; ++v) {
+        const int c = c0 + v * (kDrawT / 64);
+        if (c >= C) break;
+        if (below[c] < kBins && (far >= rest || kb >= rest)) any[v] = 1;
+        for (int j = max(sure - below[c], 0) + 64 + lane; j <= far - below[c]; j += 64)
+          any[v] |= tokens_in((at + c) * kBins + min(j, kRest));
+        const u64 all = wave_total(sum[v]);
+        if (lane == 0) kept[c] = all;
+        if (__any(any[v] != 0) && lane == 0) scan[atomicAdd(&scans, 1u)] = (uint16_t)c;
+      }
     }
     __syncthreads();
-    // their tokens: first by bounds in fp32, a little wide, then by their bins
-    auto bound = [&](int bin, double sign) {
-      const double v = (top - (double)bin) / s.bins;
-      return mx < INFINITY ? (float)(v + sign * (1e-6 * fabs(v) + 0.01 / s.bins)) : (float)sign * INFINITY;
+    // their tokens: first by an interval in fp32, a little wide, then by their bins.  Down to the rest it is everything
+    // finite (-inf is no token, nor what is read past the row).
+    auto interval = [&](int from, int to, float& mid, float& half) {
+      const double lo = (top - (double)to) / s.bins, hi = fmin((top - (double)from + 1.0) / s.bins, (double)mx);
+      const double m = 0.5 * (lo + hi), h = 0.5 * (hi - lo);
+      const bool all = to >= rest || !(mx < INFINITY) || !(fabs(m) + h < 1e38);
+      mid = all ? 0.f : (float)m;
+      half = all ? INFINITY : (float)(h + 1e-6 * (fabs(m) + h) + 0.01 / s.bins);
     };
-    const float lo1 = far >= rest ? -INFINITY : bound(far, -1.0), hi1 = sure > 0 ? bound(sure - 1, 1.0) : INFINITY;
-    const float lo2 = kb < 0 ? INFINITY : kb >= rest ? -INFINITY : bound(kb, -1.0);
-    const float hi2 = kb < 0 ? -INFINITY : kb > 0 ? bound(kb - 1, 1.0) : INFINITY;
-    constexpr int U = 4;                   // reads in flight
+    float mid1, half1, mid2, half2;
+    interval(sure, far, mid1, half1);
+    interval(max(kb, 0), max(kb, 0), mid2, half2);
+    const bool two = kb > far;             // top-k's bin lies apart
+    constexpr int U = 4;                   // groups in flight: 32 logits a lane
     const int shift = __builtin_ctz(a.chunk / 8), jobs = (int)scans << shift;
+    uint32_t* const found_at = (uint32_t*)place;                // (indices first: the logits follow)
     for (int j0 = tid - (tid & 63); j0 < jobs; j0 += U * kDrawT) {              // (whole waves)
       float x[U][8];
       int at_[U];
@@ -627,51 +664,67 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
       for (int v = 0; v < U; ++v) {
         const int j = min(j0 + (tid & 63) + v * kDrawT, jobs - 1);
         at_[v] = scan[j >> shift] * a.chunk + 8 * (j & ((1 << shift) - 1));
-        logits8<TYPE>(a, p, vec, at_[v], x[v]);
       }
-      uint32_t hits = 0;
+      logits8<TYPE>(a, p, vec, at_, x);
+      uint32_t hits = 0;                   // logit e of read v at bit 8 v + 7 - e
 #pragma unroll
-      for (int v = 0; v < U; ++v) {
+      for (int v = U - 1; v >= 0; --v) {
         uint32_t h = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = x[v][e];
-          h |= (uint32_t)((((y >= lo1) & (y <= hi1)) | ((y >= lo2) & (y <= hi2))) & (y > -INFINITY)) << e;
+        for (int e = 0; e < 8; ++e) h = h + h + (uint32_t)(fabsf(x[v][e] - mid1) <= half1);
+        if (two) {
+          uint32_t h2 = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h2 = h2 + h2 + (uint32_t)(fabsf(x[v][e] - mid2) <= half2);
+          h |= h2;
         }
-        hits |= (j0 + (tid & 63) + v * kDrawT < jobs ? h : 0u) << (8 * v);
+        hits = hits << 8 | (j0 + (tid & 63) + v * kDrawT < jobs ? h : 0u);
       }
       if (!__any(hits != 0)) continue;
       uint32_t all, from = wave_prefix(__builtin_popcount(hits), tid & 63, all);
       uint32_t base = 0;
       if ((tid & 63) == 0) base = atomicAdd(&listed, all);
       from += __builtin_amdgcn_readfirstlane(base);
+      while (hits) {
+        const int bit = __builtin_ctz(hits), v = bit >> 3;
+        int i = at_[0];
 #pragma unroll
-      for (int v = 0; v < U; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (hits >> (8 * v + e) & 1) {
-            if (from < kList) place[from] = place_of(x[v][e], at_[v] + e);
-            ++from;
-          }
+        for (int k = 1; k < U; ++k) i = v == k ? at_[k] : i;
+        if (from < kList) found_at[from] = i + 7 - (bit & 7);
+        ++from;
+        hits &= hits - 1;
+      }
     }
     __syncthreads();
     const bool whole = listed <= kList;
     const int found = whole ? (int)listed : 0;
     __syncthreads();
-    // what is found by the bounds alone leaves the list again; what only min-p decides is counted at once
     if (tid == 0 && whole) listed = 0;
+    u64 pl[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = tid + e * kDrawT;
+      const int k = i < found ? (int)found_at[i] : -1;
+      const float y = k >= 0 && k < a.vocab ? logit<TYPE>(p, k) : -INFINITY;
+      pl[e] = y > -INFINITY ? place_of(y, k) : 0;
+    }
     __syncthreads();
+    // what is found by the bounds alone leaves the list again; what only min-p decides is counted at once
     uint32_t mine_n = 0, mine_k = 0;
-    for (int i = tid; i < found; i += kDrawT) {
-      const float y = unordered((uint32_t)(place[i] >> 32));
-      const int b = min(bin_of(y, top, s.bins), rest);
-      if ((b >= r_first && b <= r_last) || b == kb) {
-        ++mine_n;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = tid + e * kDrawT;
+      if (i < found) {
+        const float y = unordered((uint32_t)(pl[e] >> 32));
+        const int b = pl[e] ? min(bin_of(y, top, s.bins), rest) : -2;
+        const bool in = (b >= r_first && b <= r_last) || b == kb;
+        mine_n += in;
         mine_k += b == kb;
-      } else {
-        const uint32_t c = ~(uint32_t)place[i] / (uint32_t)a.chunk;
-        if (b >= sure && b < r_first && passes_min(y)) atomicAdd(&kept[c], own_mass(y, cmx[c]));
-        place[i] = 0;
+        if (!in && b >= sure && b < r_first && passes_min(y)) {
+          const uint32_t c = ~(uint32_t)pl[e] / (uint32_t)a.chunk;
+          atomicAdd(&kept[c], own_mass(y, cmx[c]));
+        }
+        place[i] = in ? pl[e] : 0;
       }
     }
     if (mine_n) atomicAdd(&listed, mine_n);
@@ -680,8 +733,8 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
     const uint32_t n = listed;
     if (!whole && min_only) {              // (a row of almost nothing else: chunk by chunk, no list)
       for (int i = 8 * tid; i < a.vocab; i += 8 * kDrawT) {
-        float x[8];
-        logits8<TYPE>(a, p, vec, i, x);
+        float x1[1][8], (&x)[8] = x1[0];
+        logits8<TYPE>(a, p, vec, {i}, x1);
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -696,8 +749,8 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
       __syncthreads();
       for (int i = 8 * tid; i < a.vocab; i += 8 * kDrawT) {
         const int c = i / a.chunk;         // (a chunk is a multiple of 8)
-        float x[8];
-        logits8<TYPE>(a, p, vec, i, x);
+        float x1[1][8], (&x)[8] = x1[0];
+        logits8<TYPE>(a, p, vec, {i}, x1);
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -799,30 +852,38 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
   u64 aim = over > 0.0 ? (u64)over : 0;
   aim = aim < kept[ch] ? aim : kept[ch] - 1;
   u64 passed = 0;
-  for (int j0 = c0; j0 < end; j0 += 8 * kDrawT) {
-    const int i = j0 + 8 * tid;
-    u64 m[8], sum = 0, all;
+  // nothing below the threshold's logit is kept (a threshold under every number: everything)
+  const uint32_t t_hi = (uint32_t)(thr >> 32);
+  const float least = t_hi > ordered(-INFINITY) ? unordered(t_hi) : -FLT_MAX;
+  constexpr int V = 2;                     // reads in flight
+  for (int j0 = c0; j0 < end; j0 += V * 8 * kDrawT) {
+    float x[V][8];
+    int at_[V];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m[e] = 0;
-    if (i < end) {
-      float x[8];
-      logits8<TYPE>(a, p, vec, i, x);
+    for (int v = 0; v < V; ++v) at_[v] = j0 + 8 * (v * kDrawT + tid);
+    logits8<TYPE>(a, p, vec, at_, x);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = j0 + 8 * (v * kDrawT + tid);
+      u64 m[8], sum = 0, all;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (x[e] > -INFINITY && place_of(x[e], i + e) >= thr && passes_min(x[e])) m[e] = own_mass(x[e], cmx[ch]);
+        m[e] = 0;
+        if (x[v][e] >= least && i < end && place_of(x[v][e], i + e) >= thr && passes_min(x[v][e]))
+          m[e] = own_mass(x[v][e], cmx[ch]);
         sum += m[e];
       }
-    }
-    u64 before = passed + block_prefix<kDrawT>(sum, red, all) - sum;
-    if (before <= aim && aim < before + sum) {
+      u64 before = passed + block_prefix<kDrawT>(sum, red, all) - sum;
+      if (before <= aim && aim < before + sum) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (before <= aim && aim < before + m[e]) finish(i + e, log((double)m[e] * f / total));
-        before += m[e];
+        for (int e = 0; e < 8; ++e) {
+          if (before <= aim && aim < before + m[e]) finish(i + e, log((double)m[e] * f / total));
+          before += m[e];
+        }
       }
+      passed += all;
+      if (passed > aim) return;
     }
-    passed += all;
-    if (passed > aim) break;
   }
 }
 
@@ -831,7 +892,7 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
 
 // Chunks of 4096 logits keep a single row's steps short; from 64 rows on the
 // rows fill the card and larger chunks write fewer bins.
-int64_t chunk_of(int64_t rows) { return rows >= 64 ? 16384 : 4096; }
+int64_t chunk_of(int64_t rows) { return rows >= 64 ? 8192 : 4096; }
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -861,7 +922,7 @@ template <int TYPE>
 void launch(const SampleArgs& a, int64_t rows, hipStream_t st) {
   const dim3 grid((unsigned)a.chunks, (unsigned)rows);
   if (a.chunk == 4096) hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 2>), grid, dim3(kT), 0, st, a);
-  else hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 8>), grid, dim3(kT), 0, st, a);
+  else hipLaunchKernelGGL((sample_chunk_kernel<TYPE, 4>), grid, dim3(kT), 0, st, a);
   hipLaunchKernelGGL(sample_draw_kernel<TYPE>, dim3((unsigned)rows), dim3(kDrawT), 0, st, a);
 }
 
