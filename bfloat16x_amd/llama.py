@@ -27,7 +27,13 @@ device-resident state:
     RMSNorm launch remains inside the stack (residual_norm; 3.15 against
     3.21 ms/token with the standalone RMSNorm launches).  norm_in_gemv, where
     every GEMV workgroup also recomputes the sum of squares itself, measured
-    no faster and is off by default.
+    no faster and is off by default;
+  * kv_bits = 4 keeps K and V in 4 bits (kv4): rotary embedding and append in
+    one launch, then attention over the codes, for prompts and for single
+    tokens; 80 bytes per token and head instead of 256 per K or V row;
+  * sample = dict(temperature=..., top_k=..., top_p=..., min_p=...) draws the
+    tokens (sampling.sample) from the uniform numbers in `uniform`, one per
+    new token, instead of taking the maximum.
 
 Shapes of the benchmark configuration (the defaults of LlamaConfig): 32
 layers, hidden 4096, FFN 14336 (SwiGLU), 32 query / 8 KV heads, head_dim 128,
@@ -43,7 +49,7 @@ import math
 import torch
 from torch import nn
 
-from . import _lib, ops
+from . import _lib, kv4, ops, sampling
 
 __all__ = ["LlamaConfig", "LlamaStack", "LlamaRunner", "rope_table", "rmsnorm", "rope_kv", "attention", "pairs8_rows",
            "attention_decode", "attention_decode_supported", "attention_decode_workspace", "layer_front_decode",
@@ -409,28 +415,47 @@ class LlamaStack(nn.Module):
 
 
 class LlamaRunner:
-    """Prefill + greedy decode over a LlamaStack whose linears are bf16
+    """Prefill + decode over a LlamaStack whose linears are bf16
     nn.Linear or BF16X modules (anything mapping [.., in] -> [.., out]).
 
     Device state: `token` (int64 [1], the next input), `state` (int32 [2]:
     position of `token`, number of tokens in `history`), `history` (int32
     [max_new]).  prefill() fills the caches with the prompt and emits the
     first token; each decode step consumes `token`, appends one token to the
-    history and advances the position."""
+    history and advances the position.
+
+    kv_bits: 16 (bf16 caches) or 4 (kv4.Kv4Cache, any max_len).  sample: None
+    (greedy) or the settings of sampling.sample; `uniform` (fp32 [max_new],
+    random from `seed`; a caller may fill it) holds the numbers that the tokens
+    are drawn with."""
 
     def __init__(self, model: LlamaStack, max_len: int, max_new: int, max_prompt: int | None = None,
-                 norm_in_gemv: bool = False, residual_norm: bool = True, layer_front: bool = True):
+                 norm_in_gemv: bool = False, residual_norm: bool = True, layer_front: bool = True,
+                 kv_bits: int = 16, sample: dict | None = None, seed: int = 0):
         cfg = model.cfg
         self.model, self.cfg = model, cfg
         dev = model.device
-        if max_len > 16384:
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 16 or 4")
+        if sample is not None and set(sample) - {"temperature", "top_k", "top_p", "min_p"}:
+            raise ValueError("sample takes temperature, top_k, top_p and min_p")
+        if max_len > 16384 and kv_bits == 16:
             raise ValueError("max_len <= 16384 (attention scores are kept in LDS)")
         self.max_len, self.max_new = int(max_len), int(max_new)
         self.max_prompt = int(max_prompt if max_prompt is not None else max_len)
         T = max(self.max_prompt, 1)
         bf = dict(dtype=torch.bfloat16, device=dev)
-        self.k_cache = torch.zeros(cfg.n_layers, cfg.n_kv_heads, self.max_len, HEAD_DIM, **bf)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.kv_bits = kv_bits
+        if kv_bits == 4:
+            self.k_cache = self.v_cache = None
+            layers = kv4.Kv4Cache.zeros(cfg.n_layers, cfg.n_kv_heads, self.max_len, HEAD_DIM, device=dev)
+            self.kv4_caches = [kv4.Kv4Cache(*(t[i:i + 1] for t in layers)) for i in range(cfg.n_layers)]
+        else:
+            self.k_cache = torch.zeros(cfg.n_layers, cfg.n_kv_heads, self.max_len, HEAD_DIM, **bf)
+            self.v_cache = torch.zeros_like(self.k_cache)
+        self.sample = dict(sample) if sample is not None else None
+        self.uniform = torch.rand(max(self.max_new, 1), dtype=torch.float32, device=dev,
+                                  generator=torch.Generator(device=dev).manual_seed(int(seed)))
         self.cos_sin = rope_table(self.max_len, cfg.rope_theta, dev)
         self.residual = torch.empty(T, cfg.hidden, **bf)
         self.normed = torch.empty(T, cfg.hidden, **bf)
@@ -446,19 +471,21 @@ class LlamaRunner:
         self.graph = None
         self._graph_logits = None
         # one-token steps fold RoPE + KV append into one attention launch per KV head
-        self.fused_decode_attention = attention_decode_supported(cfg.n_heads, cfg.n_kv_heads, self.max_len)
+        self.fused_decode_attention = kv_bits == 16 and attention_decode_supported(cfg.n_heads, cfg.n_kv_heads,
+                                                                                   self.max_len)
         self.dec_ws = (attention_decode_workspace(cfg.n_heads, cfg.n_kv_heads, self.max_len, dev)
                        if self.fused_decode_attention else None)
         # norm_in_gemv: decode with the RMSNorms folded into the following GEMVs (bf16x_gemv_norm).  Off by
         # default: each of the ~900 workgroups of a GEMV recomputes the norm of the whole row before its
         # first weight row, which costs as much as the standalone RMSNorm launch it saves (measured: gate_up
         # 40.2 us vs 32.5 + 5.3 us, qkv 14.7 vs 15.3 us; 3.43 vs 3.37 ms/token)
-        self.fused_norm = bool(norm_in_gemv) and self.fused_decode_attention and all(
+        one_call = self.fused_decode_attention or kv_bits == 4
+        self.fused_norm = bool(norm_in_gemv) and one_call and all(
             _norm_gemv_ok(lay.qkv) and _swiglu_gemv_ok(lay.gate_up) for lay in model.layers)
         # residual_norm (default, BF16X stacks): the o and down GEMVs add their output to the residual stream
         # and leave per-workgroup sums of squares (bf16x_gemv_residual); the next qkv / gate_up GEMV normalises
         # its input from them (bf16x_gemv_prenormed): no RMSNorm launch inside the stack, 5 launches per layer
-        self.res_norm = (bool(residual_norm) and not self.fused_norm and self.fused_decode_attention and all(
+        self.res_norm = (bool(residual_norm) and not self.fused_norm and one_call and all(
             _norm_gemv_ok(lay.qkv) and _swiglu_gemv_ok(lay.gate_up) and _residual_gemv_ok(lay.o)
             and _residual_gemv_ok(lay.down) for lay in model.layers))
         self.res_a = torch.empty(cfg.hidden, **bf)
@@ -476,13 +503,36 @@ class LlamaRunner:
         # the step (the graph repeats it), must differ: c = 0, 1, 0, 1, ..., and 2 for the last launch
         lay0 = model.layers[0]
         cus = torch.cuda.get_device_properties(dev).multi_processor_count
-        self.front = bool(layer_front) and self.res_norm and cfg.n_layers >= 3 and layer_front_supported(
+        self.front = bool(layer_front) and self.res_norm and kv_bits == 16 and cfg.n_layers >= 3 and layer_front_supported(
             cfg.n_heads, cfg.n_kv_heads, self.max_len, lay0.qkv.out_features, lay0.qkv.in_features, cus) and \
             lay0.o.in_features == lay0.qkv.in_features
         if self.front:
             self.front_sync = layer_front_sync(dev, 3)
             self.front_buf = layer_front_buffers(cfg.n_layers - 1)
         self._prompt_len = 0
+
+    def _attend(self, i: int, qkv: torch.Tensor, pos: torch.Tensor, T: int) -> None:
+        """RoPE, cache append and attention of layer i for T tokens from pos[0]
+        on, into self.attn."""
+        H, KV = self.cfg.n_heads, self.cfg.n_kv_heads
+        if self.kv_bits == 4:
+            q, k, v = qkv.view(1, T, H + 2 * KV, HEAD_DIM).split([H, KV, KV], dim=2)
+            c = self.kv4_caches[i]
+            q = kv4.append(k, v, c, pos[:1], q=q, cos_sin=self.cos_sin)
+            kv4.attention(q, c, pos[:1], out=self.attn[:T].view(1, T, H, HEAD_DIM))
+        elif T == 1 and self.fused_decode_attention:
+            attention_decode(qkv, pos, self.cos_sin, H, KV, self.k_cache[i], self.v_cache[i], self.attn, self.dec_ws)
+        else:
+            rope_kv(qkv, pos, self.cos_sin, H, KV, self.q, self.k_cache[i], self.v_cache[i])
+            attention(self.q, self.k_cache[i], self.v_cache[i], pos, H, KV, self.attn, tokens=T)
+
+    def _next_token(self) -> None:
+        """The next token from self.logits: drawn, or the maximum."""
+        if self.sample is not None:
+            sampling.sample(self.logits, self.uniform, token=self.token, state=self.state, history=self.history,
+                            **self.sample)
+        else:
+            greedy(self.logits, self.token, self.state, self.history, self.greedy_ws)
 
     def _decode_fused(self, pos: torch.Tensor, ids: torch.Tensor):
         """One decode token with every RMSNorm after the first folded into the
@@ -491,7 +541,6 @@ class LlamaRunner:
         down GEMV (5 launches).  The residual stream alternates between two
         one-row buffers (a GEMV stores x + residual to the other one)."""
         cfg, m = self.cfg, self.model
-        H, KV = cfg.n_heads, cfg.n_kv_heads
         R = (self.res_a, self.res_b)
         cur = 0
         rmsnorm(m.embed, m.layers[0].attn_norm, self.normed, R[0], row_idx=ids, flags=NORM_STORE, eps=cfg.eps)
@@ -505,7 +554,7 @@ class LlamaRunner:
                                           q._delta, q._emax, q.out_features, q.in_features, plan=q._plan,
                                           out=self.qkv_buf)
                 cur = 1 - cur
-            attention_decode(qkv, pos, self.cos_sin, H, KV, self.k_cache[i], self.v_cache[i], self.attn, self.dec_ws)
+            self._attend(i, qkv, pos, 1)
             o = lay.o(self.attn[0])
             g = lay.gate_up
             ops.bf16x_gemv_norm(o, R[cur], lay.mlp_norm, R[1 - cur], cfg.eps, g._sign, g._mant, g._delta, g._emax,
@@ -543,8 +592,7 @@ class LlamaRunner:
                     qkv = ops.bf16x_gemv_prenormed(R[cur], lay.attn_norm, cfg.eps, self.slots, self.n_slots_down,
                                                    q._sign, q._mant, q._delta, q._emax, q.out_features, q.in_features,
                                                    plan=q._plan, out=self.qkv_buf)
-                attention_decode(qkv, pos, self.cos_sin, H, KV, self.k_cache[i], self.v_cache[i], self.attn,
-                                 self.dec_ws)
+                self._attend(i, qkv, pos, 1)
                 ops.bf16x_gemv_residual(self.attn[0], R[cur], R[1 - cur], self.slots, o._sign, o._mant, o._delta,
                                         o._emax, o.out_features, o.in_features, plan=o._plan, out=self.proj_out)
             cur = 1 - cur
@@ -559,7 +607,6 @@ class LlamaRunner:
     # one pass over the stack for `T` tokens starting at position pos[0]
     def _layers(self, T: int, pos: torch.Tensor, ids: torch.Tensor):
         cfg, m = self.cfg, self.model
-        H, KV = cfg.n_heads, cfg.n_kv_heads
         one = T == 1
 
         def rows(buf):                    # decode feeds 1-D rows: the linears take the GEMV path
@@ -573,12 +620,7 @@ class LlamaRunner:
             else:
                 rmsnorm(prev, lay.attn_norm, self.normed, self.residual, flags=NORM_ADD | NORM_STORE, eps=cfg.eps)
             qkv = lay.qkv(rows(self.normed))
-            if one and self.fused_decode_attention:
-                attention_decode(qkv, pos, self.cos_sin, H, KV, self.k_cache[i], self.v_cache[i], self.attn,
-                                 self.dec_ws)
-            else:
-                rope_kv(qkv, pos, self.cos_sin, H, KV, self.q, self.k_cache[i], self.v_cache[i])
-                attention(self.q, self.k_cache[i], self.v_cache[i], pos, H, KV, self.attn, tokens=T)
+            self._attend(i, qkv, pos, T)
             o = lay.o(rows(self.attn))
             rmsnorm(o, lay.mlp_norm, self.normed, self.residual, flags=NORM_ADD | NORM_STORE, eps=cfg.eps)
             gu_mod = lay.gate_up
@@ -594,7 +636,7 @@ class LlamaRunner:
     def _head(self, last_down: torch.Tensor, last_res: torch.Tensor):
         rmsnorm(last_down, self.model.norm, self.normed, last_res, flags=NORM_ADD, eps=self.cfg.eps)
         self.logits = self.model.lm_head(self.normed[0])
-        greedy(self.logits, self.token, self.state, self.history, self.greedy_ws)
+        self._next_token()
 
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor) -> None:
@@ -622,7 +664,7 @@ class LlamaRunner:
             h = self._decode_resnorm(self.state, self.token)
             rmsnorm(h, self.model.norm, self.normed, eps=self.cfg.eps)
             self.logits = self.model.lm_head(self.normed[0])
-            greedy(self.logits, self.token, self.state, self.history, self.greedy_ws)
+            self._next_token()
             return
         down = self._layers(1, self.state, self.token)
         self._head(down, self.residual[0])
@@ -677,7 +719,7 @@ class LlamaRunner:
                                "layer_front=False to use the separate launches")
 
     def generate(self, ids: torch.Tensor, n_new: int, graph: bool = True) -> list:
-        """Greedy decode of n_new tokens after the prompt; the token ids."""
+        """n_new tokens after the prompt (greedy, or drawn with `sample`); the token ids."""
         if not (1 <= n_new <= self.max_new):
             raise ValueError(f"n_new must be in [1, {self.max_new}]")
         self.prefill(ids)
@@ -688,4 +730,5 @@ class LlamaRunner:
         """K and V bytes the attention of one decode step reads at the mean
         context length of a generation from the current prompt."""
         ctx = self._prompt_len + self.max_new / 2
-        return int(2 * self.cfg.n_layers * self.cfg.n_kv_heads * ctx * HEAD_DIM * 2)
+        row = HEAD_DIM * 2 if self.kv_bits == 16 else HEAD_DIM // 2 + HEAD_DIM // 32 * 4
+        return int(2 * self.cfg.n_layers * self.cfg.n_kv_heads * ctx * row)
