@@ -107,10 +107,17 @@ __device__ __forceinline__ void store8(void* p, int64_t i, const float (&x)[8]) 
   }
 }
 
+// r / n by inv = 2^32 / n rounded up (0 for n = 1): at most one too many for r < 2^30.
+__device__ __forceinline__ uint32_t quotient(uint32_t r, uint32_t n, uint32_t inv) {
+  if (n == 1) return r;
+  const uint32_t q = __umulhi(r, inv);
+  return q * n > r ? q - 1 : q;
+}
+uint32_t inverse(int64_t n) { return n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0u; }
+
 struct AppendArgs {
   const void *q, *k, *v;
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
-  int64_t rows;                            // batch x tokens x heads of a token
   int tokens, H, KV, max_len;
   const int32_t* pos;
   const float* cos_sin;
@@ -119,75 +126,78 @@ struct AppendArgs {
   uint32_t *kc, *ks, *vc, *vs;
 };
 
+// A workgroup per token; its rows (heads of q, k and v) are taken 256 / LR at a
+// time, by gridDim.z workgroups where there are few tokens.  The table's row is
+// read once per lane for all of them.
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
 #pragma clang fp contract(off)             // the rotation's products are rounded one by one, as its definition says
-  constexpr int LR = D / 8;                // lanes per row
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;
-  const int l = threadIdx.x % LR;
-  if (row >= a.rows) return;               // whole rows: the lanes of a group leave together
-  const int heads = a.H + 2 * a.KV;
-  const int64_t bt = row / heads;
-  const int h = (int)(row - bt * heads), b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
-  const int64_t p = (int64_t)a.pos[b] + t;
-  const bool is_q = h < a.H, is_k = !is_q && h < a.H + a.KV;
-  const int hk = is_q ? h : is_k ? h - a.H : h - a.H - a.KV;
-  if (!is_q && (p < 0 || p >= a.max_len)) return;
-  const void* src = is_q ? a.q : is_k ? a.k : a.v;
-  const int64_t off = is_q ? b * a.q_sb + t * a.q_st + hk * a.q_sh
-                           : is_k ? b * a.k_sb + t * a.k_st + hk * a.k_sh : b * a.v_sb + t * a.v_st + hk * a.v_sh;
-  float x[8];
-  load8<TYPE>(src, off + 8 * l, x);
-  if (a.cos_sin && (is_q || is_k)) {
-    float y[8];
-    load8<TYPE>(src, off + 8 * (l ^ (LR / 2)), y);
+  constexpr int LR = D / 8, NR = 256 / LR; // lanes per row, rows at a time
+  const int l = threadIdx.x % LR, t = blockIdx.x, heads = a.H + 2 * a.KV;
+  const int64_t b = blockIdx.y, bt = b * a.tokens + t, p = (int64_t)a.pos[b] + t;
+  const bool upper = l >= LR / 2, inside = p >= 0 && p < a.max_len;
+  f4 cs[4];
+  if (a.cos_sin) {
     const int64_t pc = p < 0 ? 0 : p >= a.cos_rows ? a.cos_rows - 1 : p;
-    const f4* cs = (const f4*)(a.cos_sin + (pc * (D / 2) + 8 * (l % (LR / 2))) * 2);
-    const bool upper = l >= LR / 2;
+    const f4* c = (const f4*)(a.cos_sin + (pc * (D / 2) + 8 * (l % (LR / 2))) * 2);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const f4 c = cs[e];
+    for (int e = 0; e < 4; ++e) cs[e] = c[e];
+  }
+  for (int h = blockIdx.z * NR + threadIdx.x / LR; h < heads; h += gridDim.z * NR) {
+    const bool is_q = h < a.H, is_k = !is_q && h < a.H + a.KV;
+    const int hk = is_q ? h : is_k ? h - a.H : h - a.H - a.KV;
+    if (!is_q && !inside) continue;        // (whole rows: the lanes of a group go together)
+    const void* src = is_q ? a.q : is_k ? a.k : a.v;
+    const int64_t off = is_q ? b * a.q_sb + t * a.q_st + hk * a.q_sh
+                             : is_k ? b * a.k_sb + t * a.k_st + hk * a.k_sh : b * a.v_sb + t * a.v_st + hk * a.v_sh;
+    float x[8];
+    load8<TYPE>(src, off + 8 * l, x);
+    if (a.cos_sin && (is_q || is_k)) {
+      float y[8];
+      load8<TYPE>(src, off + 8 * (l ^ (LR / 2)), y);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float own = x[2 * e + u] * c[2 * u], other = y[2 * e + u] * c[2 * u + 1];
-        x[2 * e + u] = upper ? own + other : own - other;
+      for (int e = 0; e < 8; ++e) {
+        const float own = x[e] * cs[e >> 1][2 * (e & 1)], other = y[e] * cs[e >> 1][2 * (e & 1) + 1];
+        x[e] = upper ? own + other : own - other;
       }
     }
-  }
-  if (is_q) {
-    store8<TYPE>(a.q_out, (bt * a.H + hk) * D + 8 * l, x);
-    return;
-  }
-  float mn = kLargest, mx = -kLargest;
+    if (is_q) {
+      store8<TYPE>(a.q_out, (bt * a.H + hk) * D + 8 * l, x);
+      continue;
+    }
+    float mn = kLargest, mx = -kLargest;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    x[e] = x[e] != x[e] ? 0.f : fminf(fmaxf(x[e], -kLargest), kLargest);
-    mn = fminf(mn, x[e]);
-    mx = fmaxf(mx, x[e]);
-  }
+    for (int e = 0; e < 8; ++e) {
+      x[e] = x[e] != x[e] ? 0.f : fminf(fmaxf(x[e], -kLargest), kLargest);
+      mn = fminf(mn, x[e]);
+      mx = fmaxf(mx, x[e]);
+    }
 #pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    mn = fminf(mn, __shfl_xor(mn, o, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  }
-  const _Float16 low = (_Float16)mn;
-  const float lowf = (float)low;
-  const _Float16 sc = (_Float16)(fmaxf(mx - lowf, 0.f) / 15.f);
-  const float scf = (float)sc;
-  uint32_t w = 0;
+    for (int o = 1; o <= 2; o <<= 1) {
+      mn = fminf(mn, __shfl_xor(mn, o, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    }
+    const _Float16 low = (_Float16)mn;
+    const float lowf = (float)low;
+    float step = fmaxf(mx - lowf, 0.f) * (1.f / 15.f);
+    asm("" : "+v"(step));                  // rounded to fp32, then to fp16: not in one v_fma_mixlo_f16
+    const _Float16 sc = (_Float16)step;
+    const float scf = (float)sc;
+    uint32_t w = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float n = scf > 0.f ? fminf(fmaxf(__builtin_rintf((x[e] - lowf) / scf), 0.f), 15.f) : 0.f;
-    w |= (uint32_t)n << (e & 1 ? 14 + 2 * e : 2 * e);
+    for (int e = 0; e < 8; ++e) {
+      const float n = scf > 0.f ? fminf(fmaxf(__builtin_rintf((x[e] - lowf) / scf), 0.f), 15.f) : 0.f;
+      w |= (uint32_t)n << (e & 1 ? 14 + 2 * e : 2 * e);
+    }
+    const int64_t out = (b * a.KV + hk) * a.max_len + p;
+    (is_k ? a.kc : a.vc)[out * LR + l] = w;
+    if ((l & 3) == 0) (is_k ? a.ks : a.vs)[out * (D / 32) + l / 4] = as_u32(h2{sc, low});
   }
-  const int64_t out = ((int64_t)b * a.KV + hk) * a.max_len + p;
-  (is_k ? a.kc : a.vc)[out * LR + l] = w;
-  if ((l & 3) == 0) (is_k ? a.ks : a.vs)[out * (D / 32) + l / 4] = as_u32(h2{sc, low});
 }
 
 struct ReadArgs {
   const uint32_t *kc, *ks, *vc, *vs;
-  int64_t rows;                            // 2 x batch x tokens x KV
+  uint32_t rows, inv;                      // tokens x KV; 2^32 / KV, rounded up
   int tokens, KV, max_len;
   const int32_t* pos;
   void *k_out, *v_out;
@@ -196,24 +206,23 @@ struct ReadArgs {
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
   constexpr int LR = D / 8;
-  int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;
+  const uint32_t row = blockIdx.x * (256 / LR) + threadIdx.x / LR;
   const int l = threadIdx.x % LR;
   if (row >= a.rows) return;
-  const bool is_k = row < a.rows / 2;
-  if (!is_k) row -= a.rows / 2;
-  const int64_t bt = row / a.KV;
-  const int h = (int)(row - bt * a.KV), b = (int)(bt / a.tokens), t = (int)(bt - (int64_t)b * a.tokens);
+  const bool is_k = blockIdx.z == 0;
+  const int t = (int)quotient(row, (uint32_t)a.KV, a.inv), h = (int)(row - t * a.KV);
+  const int64_t b = blockIdx.y;
   const int64_t p = (int64_t)a.pos[b] + t;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (p >= 0 && p < a.max_len) {
-    const int64_t at = ((int64_t)b * a.KV + h) * a.max_len + p;
+    const int64_t at = (b * a.KV + h) * a.max_len + p;
     const uint32_t w = (is_k ? a.kc : a.vc)[at * LR + l];
     const h2 s = as_h2((is_k ? a.ks : a.vs)[at * (D / 32) + l / 4]);
     const float sc = (float)s.x, low = (float)s.y;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fmaf(sc, (float)((w >> (e & 1 ? 14 + 2 * e : 2 * e)) & 15u), low);
   }
-  store8<TYPE>(is_k ? a.k_out : a.v_out, row * D + 8 * l, x);
+  store8<TYPE>(is_k ? a.k_out : a.v_out, (b * a.rows + row) * D + 8 * l, x);
 }
 
 // ---------------------------------------------------------------------------
@@ -239,9 +248,7 @@ struct AttnArgs {
 
 // Token of a query row.
 __device__ __forceinline__ int token_of(const AttnArgs& a, int r) {
-  if (a.G == 1) return r;
-  const int t = (int)__umulhi((uint32_t)r, a.g_inv);            // at most one too many for r < 2^30
-  return t * a.G > r ? t - 1 : t;
+  return (int)quotient((uint32_t)r, (uint32_t)a.G, a.g_inv);
 }
 
 // A value that is the same in every lane, known to the compiler as such.
@@ -997,13 +1004,14 @@ extern "C" int bf16x_kv4_append(const void* q, int64_t q_sb, int64_t q_st, int64
     return BF16X_EARG;
   if (batch == 0 || tokens == 0) return BF16X_OK;
   const int H = q ? (int)n_heads : 0;
-  AppendArgs a{q, k, v, q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, batch * tokens * (H + 2 * n_kv_heads),
-               (int)tokens, H, (int)n_kv_heads, (int)max_len, pos, cos_sin, cos_rows, q_out, (uint32_t*)k_codes,
-               (uint32_t*)k_scales, (uint32_t*)v_codes, (uint32_t*)v_scales};
-  const int64_t blocks = (a.rows * (head_dim / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return BF16X_ESHAPE;
+  if (batch > 65535) return BF16X_ESHAPE;
+  AppendArgs a{q, k, v, q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, (int)tokens, H, (int)n_kv_heads,
+               (int)max_len, pos, cos_sin, cos_rows, q_out, (uint32_t*)k_codes, (uint32_t*)k_scales,
+               (uint32_t*)v_codes, (uint32_t*)v_scales};
+  const int64_t at_once = 2048 / head_dim, turns = (H + 2 * n_kv_heads + at_once - 1) / at_once;
+  const dim3 grid((unsigned)tokens, (unsigned)batch, tokens * batch >= 1024 ? 1u : (unsigned)std::min<int64_t>(turns, 65535));
 #define APPEND(D, T) \
-  hipLaunchKernelGGL((kv4_append_kernel<D, T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
+  hipLaunchKernelGGL((kv4_append_kernel<D, T>), grid, dim3(256), 0, (hipStream_t)stream, a)
   if (head_dim == 128) {
     if (type == BF16X_BF16) APPEND(128, BF16X_BF16);
     else if (type == BF16X_F16) APPEND(128, BF16X_F16);
@@ -1029,11 +1037,12 @@ extern "C" int bf16x_kv4_read(const uint8_t* k_codes, const uint16_t* k_scales, 
       !aligned16(k_out) || !aligned16(v_out))
     return BF16X_EARG;
   if (batch == 0 || tokens == 0) return BF16X_OK;
+  const int64_t rows = tokens * n_kv_heads;
+  if (rows >= (1 << 30) || batch > 65535) return BF16X_ESHAPE;
   ReadArgs a{(const uint32_t*)k_codes, (const uint32_t*)k_scales, (const uint32_t*)v_codes, (const uint32_t*)v_scales,
-             2 * batch * tokens * n_kv_heads, (int)tokens, (int)n_kv_heads, (int)max_len, pos, k_out, v_out};
-  const int64_t blocks = (a.rows * (head_dim / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return BF16X_ESHAPE;
-#define READ(D, T) hipLaunchKernelGGL((kv4_read_kernel<D, T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
+             (uint32_t)rows, inverse(n_kv_heads), (int)tokens, (int)n_kv_heads, (int)max_len, pos, k_out, v_out};
+  const dim3 grid((unsigned)((rows * (head_dim / 8) + 255) / 256), (unsigned)batch, 2);
+#define READ(D, T) hipLaunchKernelGGL((kv4_read_kernel<D, T>), grid, dim3(256), 0, (hipStream_t)stream, a)
   if (head_dim == 128) {
     if (type == BF16X_BF16) READ(128, BF16X_BF16);
     else if (type == BF16X_F16) READ(128, BF16X_F16);
@@ -1078,7 +1087,7 @@ extern "C" int bf16x_kv4_attention(const void* q, int64_t q_sb, int64_t q_st, in
   // a window of max_len + tokens keys or more bounds nothing
   const int64_t win = std::min<int64_t>(window, 0x7FFFFFFF);
   AttnArgs a{(const uint16_t*)q, q_sb, q_st, q_sh, (int)batch, (int)tokens, (int)n_heads, (int)n_kv_heads, (int)G,
-             (int)max_len, (int)rows, cut.tiles, cut.splits, (int)win, scale, G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0u, k_codes, (const uint32_t*)k_scales,
+             (int)max_len, (int)rows, cut.tiles, cut.splits, (int)win, scale, inverse(G), k_codes, (const uint32_t*)k_scales,
              v_codes, (const uint32_t*)v_scales, pos, start, (uint16_t*)out, (float*)workspace};
   const hipStream_t st = (hipStream_t)stream;
   const bool bf = type == BF16X_BF16;

@@ -211,9 +211,9 @@ int bf16x_greedy(const uint16_t* logits, int64_t vocab, int64_t* token, int32_t*
  *  - scales  fp16 [batch][n_kv_heads][max_len][head_dim / 32][2]: (scale,
  *            minimum) of each group of 32 consecutive values of a row
  *  A value is minimum + scale * code, code 0 .. 15.  A group is quantised as
- *    minimum = fp16(min x), scale = fp16(max(0, max x - minimum) / 15),
+ *    minimum = fp16(min x), scale = fp16(max(0, max x - minimum) * (1 / 15)),
  *    code = round((x - minimum) / scale), half to even, cut to 0 .. 15 (0 where
- *    the scale is 0), in fp32.
+ *    the scale is 0), in fp32 (1 / 15 rounded to fp32).
  *  Values are cut to +-61440 first and a NaN counts as 0, so scales and minima
  *  written here are always finite, and so is every value in fp16.
  *  The codes of values 8w .. 8w + 7 of a row are its 4-byte word w, value

@@ -19,7 +19,7 @@ def quantise(x):
     g = x.reshape(*x.shape[:-1], -1, 32)
     low = g.min(-1).astype(np.float16)
     lowf = low.astype(np.float32)
-    scale = (np.maximum(g.max(-1) - lowf, np.float32(0)) / np.float32(15)).astype(np.float16)
+    scale = (np.maximum(g.max(-1) - lowf, np.float32(0)) * np.float32(1 / 15)).astype(np.float16)
     s = scale.astype(np.float32)[..., None]
     with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
         n = np.rint((g - lowf[..., None]) / s)

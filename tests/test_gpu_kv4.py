@@ -94,6 +94,20 @@ def test_append_rotates_k_and_q(dim, dtype):
         assert np.array_equal(got.cpu().numpy(), want)
 
 
+def test_many_fp32_rows():
+    """Enough rows for values at the borders of a scale's and a code's rounding."""
+    B, T, KV, D = 1, 3000, 4, 128
+    k, v = (_rand(B, T, KV, D, seed=s, dtype=FP) for s in (50, 51))
+    t = _table(T, D)
+    c = kv4.Kv4Cache.zeros(B, KV, T, D, device=DEV)
+    kv4.append(k.to(DEV), v.to(DEV), c, _i32([0]), cos_sin=t.to(DEV))
+    kr = serve.rotate(k.numpy(), t.numpy(), np.arange(T)[None])
+    for src, codes, scales in ((kr, c.k, c.k_scale), (v.numpy(), c.v, c.v_scale)):
+        n, s, m = serve.quantise(src)
+        assert np.array_equal(scales.cpu().numpy(), np.stack([s, m], -1).swapaxes(1, 2))
+        assert np.array_equal(codes.cpu().numpy(), serve.pack(n).swapaxes(1, 2))
+
+
 def test_quantiser_edges():
     """Constant groups, zeros, an outlier, tiny and huge values, infinities and NaN."""
     x = torch.zeros(1, 8, 1, 64)
