@@ -180,6 +180,32 @@ def test_attention(shape, dtype):
     _check_attention(q, cache, vals, pos, got)
 
 
+@pytest.mark.parametrize("tile", [16, 64, 128])
+@pytest.mark.parametrize("split", [1, 2, 3, 7, 128])
+@pytest.mark.parametrize("shape", [(1, 1, 4, 2, 128, 333), (2, 9, 6, 2, 64, 130), (2, 75, 4, 2, 128, 700)], ids=str)
+def test_every_tile_and_split(shape, tile, split, tune):
+    """Each kernel on each kind of call, the keys cut into more ranges than there are steps among it."""
+    B, T, H, KV, D, L = shape
+    tune(kv4_tile=tile, kv4_split=split)
+    q = _rand(B, T, H, D, seed=60)
+    cache, vals = _cache(_rand(B, KV, L, D, seed=61, dtype=FP), _rand(B, KV, L, D, seed=62, dtype=FP))
+    pos, start = [L - T, 37][:B], [3, 50][:B]
+    got = kv4.attention(q.to(DEV), cache, _i32(pos), start=_i32(start))
+    _check_attention(q, cache, vals, pos, got, start=start)
+
+
+def test_batch_of_many_lengths():
+    """More sequences than a wave has lanes, from one key to thousands: each gets its own steps."""
+    B, H, KV, D, L = 70, 4, 2, 64, 4096
+    q = _rand(B, 1, H, D, seed=63)
+    cache, vals = _cache(_rand(B, KV, L, D, seed=64, dtype=FP), _rand(B, KV, L, D, seed=65, dtype=FP))
+    pos = [(L - 1) * i * i // (B - 1) ** 2 for i in range(B)]
+    pos[5] = -1
+    got = kv4.attention(q.to(DEV), cache, _i32(pos))
+    _check_attention(q, cache, vals, pos, got)
+    assert (got[5] == 0).all()
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 8, 2, 128, 300), (4, 6, 6, 2, 64, 300), (4, 90, 4, 1, 128, 300)], ids=str)
 @pytest.mark.parametrize("window", [0, 1, 7, 64, 1000])
 def test_masks(shape, window):

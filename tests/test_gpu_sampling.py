@@ -82,6 +82,31 @@ def test_ties(kw, levels):
     _check(x, u, sampling.sample(x.to(DEV), u.to(DEV), **kw), **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(top_k=700), dict(top_p=0.4), dict(top_k=1500, top_p=0.9), dict(top_k=5, min_p=0.9),
+                                dict(min_p=0.999)], ids=str)
+@pytest.mark.parametrize("vocab", [300, 513, 1000, 2047, 4096, 4097])
+def test_ties_of_every_list_length(kw, vocab):
+    """Rows of one value, and of one value and a few larger ones: lists sorted by counting, bitonically, and too long."""
+    x = torch.zeros(5, vocab)
+    x[1, ::97] = 0.5
+    x[2] = -7.25
+    x[3, vocab // 2:] = -30.0
+    x[4, 3] = 9.0
+    u = torch.tensor([0.0, 0.3, 0.999, 0.5, 0.77])
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(x.to(dtype), u, sampling.sample(x.to(DEV, dtype), u.to(DEV), **kw), **kw)
+
+
+@pytest.mark.parametrize("spread", [0.01, 0.3, 12.0, 100.0])
+def test_spreads(spread):
+    """Flat rows (few bins), steep ones (most tokens below all bins)."""
+    for dtype in TYPES:
+        x, u = _logits(8, 9001, 11, dtype, spread=spread)
+        for kw in (dict(), dict(top_k=64), dict(top_p=0.97), dict(temperature=0.05, top_k=5000, top_p=0.99),
+                   dict(temperature=20.0, top_p=0.9, min_p=0.3), dict(min_p=1e-5)):
+            _check(x, u, sampling.sample(x.to(DEV), u.to(DEV), **kw), **kw)
+
+
 def test_masked_and_special_rows():
     vocab = 1031
     x, _ = _logits(10, vocab, 6, torch.float32)
