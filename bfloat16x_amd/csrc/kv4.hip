@@ -270,10 +270,11 @@ __device__ __forceinline__ uint32_t out2(float a, float b) {
   return BF ? f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16) : as_u32(h2{(_Float16)a, (_Float16)b});
 }
 
-// The query operand of a lane: 8 N values of its row brought to fp16 by the power of two that puts the row's largest value (over the 4 lanes of
-// the row) into [1, 2), with the sign of `scale`; returns what a product's sum
-// is to be multiplied with for a score in powers of two, a positive number.
-// Exact for every value within 2^-14 of the row's largest.
+// The query operand of a lane: 8 N values of its row brought to fp16 by the power
+// of two that puts the row's largest value (over the 4 lanes of the row) into
+// [1, 2), with the sign of `scale`; returns what a product's sum is to be
+// multiplied with for a score in powers of two, a positive number.  Exact for
+// every value within 2^-14 of the row's largest.
 template <bool BF, int N>
 __device__ __forceinline__ float load_query(const u32x4 (&raw)[N], bool valid, float scale, h8 (&qb)[N]) {
   us2 big = {0, 0};                        // largest magnitude as bits: ascending for both types
@@ -952,6 +953,21 @@ bool rows_aligned(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t siz
 
 // How the work of an attention call is cut: tiles of 16 query rows (few rows),
 // 64 or 128, and splits of their keys so that a small call still fills the card.
+// (Times in us in a graph, 32 heads on 8 of 128 values, one sequence where none
+// is named.)
+//  * 16 rows a tile up to 64 rows: 16 tokens at 4096 keys 13 (64 rows: 20), 24
+//    tokens 18 (22), but 8 sequences of 16 tokens 38 (35).
+//  * 64 rows a tile until two workgroups of them per CU are reached, 128 beyond:
+//    1024 tokens of a prompt 30 (128 rows: 36), 1536 48 (50), 2048 76 (64).
+//  * Splits until two workgroups per CU are reached: 32 sequences of up to 8192
+//    keys in 2 splits 46, in 1 55, in 8 53; 64 of 2048 in 1 26, in 2 35, in 4 46.
+//  * A split has 256 keys or more for single tokens (4096 keys: 16 splits 9.3, 8
+//    10.6, 4 13), 512 in long caches (16384 keys: 32 splits 13, 64 13.7) and for
+//    wide tiles; and twice as many keys as there are rows, whose partial results
+//    are written and read once per split (256 tokens at 8192 keys: 4 splits 92, 1
+//    163; at 1024 keys: 2 splits 40, 1 25).
+//  * Up to 1024 keys the join of few rows costs what it saves (640 keys: 7.5
+//    without splits, 9.7 in 2, 8.3 in 8; 16 sequences of 1024: 11 and 13 in 2).
 struct Cut {
   int rows, tiles, splits;
 };
@@ -960,12 +976,13 @@ Cut cut_of(int64_t batch, int64_t rows, int64_t tokens, int64_t KV, int64_t max_
   const int64_t wide = batch * KV * ((rows + 127) / 128);
   const int64_t tile = forced == 16 || forced == 64 || forced == 128 ? forced
                        : rows <= 64                                  ? 16
-                       : wide < 256                                  ? 64
+                       : wide <= 256                                 ? 64
                                                                      : 128;
   const int64_t keys = window > 0 ? std::min(max_len, window + tokens) : max_len;
   const int64_t tiles = (rows + tile - 1) / tile, wgs = std::max<int64_t>(batch * KV * tiles, 1);
-  int64_t want = std::min(tile == 16 ? 2048 / wgs : 512 / wgs, (keys + 511) / 512);
-  if (tile == 16 && keys <= 1536) want = 1;
+  const int64_t share = std::max<int64_t>(2 * rows, tile == 16 && keys <= 8192 ? 256 : 512);
+  int64_t want = std::min(512 / wgs, (keys + share - 1) / share);
+  if (tile == 16 && keys <= 1024) want = 1;
   if (split > 0) want = split;
   want = std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
   return {(int)tile, (int)tiles, (int)want};
