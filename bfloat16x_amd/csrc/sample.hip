@@ -37,7 +37,12 @@ constexpr int kGroup = 16;                // bins of a group, which all chunks c
 constexpr int kGroups = kBins / kGroup + 1;
 constexpr int kOpen = kBins / kGroup - 1; // groups of a row; the tokens below them are its rest
 constexpr int kList = 4096;               // tokens of the thresholds' bins that are sorted in LDS
-constexpr int kRanked = 512;              // as many are sorted by counting, more bitonically
+// A list of kRanked tokens is sorted by counting alone; a longer one by kCells
+// cells of its range if none has more than kFull tokens (128 rows of mixed
+// settings 88 us; bitonically, which very uneven lists are left to, 96).
+constexpr int kRanked = 512;
+constexpr int kCells = 2048;
+constexpr int kFull = 64;
 constexpr int kMaxChunks = 256;
 constexpr int kT = 256;                   // threads per chunk
 constexpr int kDrawT = 512;               // threads per row
@@ -758,7 +763,7 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
         if (sum) atomicAdd(&kept[c], sum);
       }
     } else if (n) {
-      // the list in descending order: by rank, or where it is long bitonic, padded with zeros
+      // the list in descending order
       if (found <= kRanked) {
         const u64 mine = tid < found ? place[tid] : 0;
         uint32_t rank = 0;
@@ -768,18 +773,85 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
         __syncthreads();
         if (mine) place[rank] = mine;
       } else {
-        int size = 2 * kRanked;
-        while (size < found) size *= 2;
-        for (int i = found + tid; i < size; i += kDrawT) place[i] = 0;
-        for (int w = 2; w <= size; w *= 2)
-          for (int h = w / 2; h >= 1; h /= 2) {
-            __syncthreads();
-            for (int i = tid; i < size / 2; i += kDrawT) {
-              const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
-              const u64 x = place[lo], y = place[hi];
-              if ((x < y) == ((lo & w) == 0)) place[lo] = y, place[hi] = x;
-            }
+        // kCells cells of the listed places' range by counting, then ranks inside a cell.  A cell falls monotonically
+        // with the logit, rounded or not; of two 16-bit logits that differ, by `gap` at least, the indices, which count
+        // 0.99 gaps from the first token to the last, cannot change the order (pos is right to 5e-4).
+        uint32_t* const cell = (uint32_t*)prefix;               // how many, then where they start
+        const int b_first = kb >= 0 ? min(r_first, kb) : r_first, b_last = max(r_last, kb);
+        const float hi = (float)fmin((top - (double)b_first + 1.0) / s.bins, (double)mx);
+        const float lo = (float)((top - (double)b_last) / s.bins);
+        float gap = 0.f;
+        if constexpr (TYPE != BF16X_F32)
+          if (hi * lo > 0.f)
+            gap = __uint_as_float(__float_as_uint(0.999f * fminf(fabsf(hi), fabsf(lo))) & 0x7F800000u) *
+                  (TYPE == BF16X_BF16 ? 0x1p-7f : 0x1p-10f);
+        const float per = (float)kCells / (hi - lo + gap);
+        const float tie = gap * per > 0.1f ? 0.99f * gap * per / (float)a.vocab : 0.f;
+        auto cell_at = [&](u64 pl) {
+          const float pos = (hi - unordered((uint32_t)(pl >> 32))) * per + (float)~(uint32_t)pl * tie;
+          return (int)fminf(fmaxf(pos, 0.f), (float)(kCells - 1));
+        };
+        bool even = b_last < rest && fabsf(hi) < 1e38f && per > 0.f && per < 1e38f;      // (the same for all threads)
+        if (even) {
+          for (int i = tid; i < kCells; i += kDrawT) cell[i] = 0;
+          __syncthreads();
+          uint32_t nth[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int i = tid + e * kDrawT;
+            pl[e] = i < found ? place[i] : 0;
+            nth[e] = pl[e] ? atomicAdd(&cell[cell_at(pl[e])], 1u) : 0;
           }
+          __syncthreads();
+          uint32_t own[kCells / kDrawT], sum = 0, most = 0, all;
+#pragma unroll
+          for (int k = 0; k < kCells / kDrawT; ++k) {
+            own[k] = cell[tid * (kCells / kDrawT) + k];
+            sum += own[k];
+            most = max(most, own[k]);
+          }
+          uint32_t from = block_prefix<kDrawT>(sum, counts, all) - sum;
+          even = !__syncthreads_or(most > kFull);
+          if (even) {
+#pragma unroll
+            for (int k = 0; k < kCells / kDrawT; ++k) {
+              cell[tid * (kCells / kDrawT) + k] = from;
+              from += own[k];
+            }
+            if (tid == 0) cell[kCells] = n;
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (pl[e]) place[cell[cell_at(pl[e])] + nth[e]] = pl[e];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (pl[e]) {
+                const int c = cell_at(pl[e]);
+                const uint32_t start = cell[c], stop = cell[c + 1];
+                nth[e] = start;
+                for (uint32_t i = start; i < stop; ++i) nth[e] += place[i] > pl[e];
+              }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (pl[e]) place[nth[e]] = pl[e];
+          }
+        }
+        if (!even) {                       // (many of one value) bitonically, padded with zeros
+          int size = 2 * kRanked;
+          while (size < found) size *= 2;
+          for (int i = found + tid; i < size; i += kDrawT) place[i] = 0;
+          for (int w = 2; w <= size; w *= 2)
+            for (int h = w / 2; h >= 1; h /= 2) {
+              __syncthreads();
+              for (int i = tid; i < size / 2; i += kDrawT) {
+                const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
+                const u64 x = place[lo], y = place[hi];
+                if ((x < y) == ((lo & w) == 0)) place[lo] = y, place[hi] = x;
+              }
+            }
+        }
       }
       __syncthreads();
       // their masses, then inclusive sums over E consecutive entries per thread

@@ -97,6 +97,20 @@ def test_ties_of_every_list_length(kw, vocab):
         _check(x.to(dtype), u, sampling.sample(x.to(DEV, dtype), u.to(DEV), **kw), **kw)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("center", [0.0, 5.0, -3.0, -20.0])
+def test_long_lists(center, dtype):
+    """Hundreds to thousands of tokens in a threshold's bins, many of them equal or a rounding step apart; the last row
+    has its larger logits at the later tokens."""
+    x, u = _logits(6, 50021, 21, torch.float32, spread=1.0)
+    x[:, : 50021 // 50] -= 3.0
+    x[5] = torch.sort(x[5]).values
+    x = (x + center).to(dtype)
+    for kw in (dict(top_p=0.7), dict(temperature=1.3, top_p=0.95), dict(top_k=20000), dict(top_k=9000, top_p=0.8),
+               dict(temperature=0.9, top_k=12000, top_p=0.9, min_p=0.01), dict(temperature=3.0, top_k=30, top_p=0.99)):
+        _check(x, u, sampling.sample(x.to(DEV), u.to(DEV), **kw), **kw)
+
+
 @pytest.mark.parametrize("spread", [0.01, 0.3, 12.0, 100.0])
 def test_spreads(spread):
     """Flat rows (few bins), steep ones (most tokens below all bins)."""
