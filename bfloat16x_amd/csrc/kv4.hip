@@ -60,8 +60,15 @@ __device__ __forceinline__ h2 scale_of(uint32_t w) { return as_h2(__builtin_amdg
 __device__ __forceinline__ h2 minimum_of(uint32_t w) { return as_h2(__builtin_amdgcn_perm(w, w, 0x03020302u)); }
 
 // ---------------------------------------------------------------------------
-// Append and read.  8 values per lane (one word of codes), so D / 8 lanes per
-// row; the 4 lanes of a group meet in two quad exchanges.
+// Append and read.  8 values per lane (one word of codes: 16 bytes of a 16-bit
+// type in one load), so D / 8 lanes per row; the 4 lanes of a group meet in two
+// quad exchanges.  Both are bound by memory, or by the launch and two dependent
+// round trips (the position, then the rows) where there are few tokens: with 32
+// + 16 heads of 128 bf16 values, 2048 tokens take 13.3 us to append (46 MB, 3.4
+// TB/s; a copy reaches 5.0) and 4.0 to read back (11 MB), one token 3.0 and 1.9.
+// Only the scale and the minimum are rounded below fp32 on the way in, to the
+// fp16 they are kept in, and the codes are taken against those rounded values,
+// so that their rounding costs no more than half a step of the code.
 
 template <int TYPE>
 __device__ __forceinline__ void values8(u32x4 r, float (&x)[8]) {
@@ -128,7 +135,8 @@ struct AppendArgs {
 
 // A workgroup per token; its rows (heads of q, k and v) are taken 256 / LR at a
 // time, by gridDim.z workgroups where there are few tokens.  The table's row is
-// read once per lane for all of them.
+// read once per lane for all of them, and no lane divides (a workgroup per 256 /
+// LR rows of any token: 15.8 us for the 2048 tokens, and 13.3 so).
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
 #pragma clang fp contract(off)             // the rotation's products are rounded one by one, as its definition says
@@ -195,6 +203,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
   }
 }
 
+// fma(scale, code, minimum), rounded once to the output's type.
 struct ReadArgs {
   const uint32_t *kc, *ks, *vc, *vs;
   uint32_t rows, inv;                      // tokens x KV; 2^32 / KV, rounded up
@@ -317,10 +326,26 @@ __device__ __forceinline__ float row_max(float x) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// The running softmax of both kernels: with M the maximum that a row's weights are
+// taken against (in powers of two), P = 2^(s - M) enters the second product as
+// fp16; M is renewed, and outputs and sum multiplied with 2^(M - M'), only when
+// the scores pass it by 8, so weights go up to 2^8, with 11 bits as ever.  Rounded
+// below fp32 are: the query, by its power of two (exact for values within 2^-14
+// of the row's largest), the cache's values, by their own fma, the weights, and
+// the output, once, to its type.  Each of them is 2^-11 at most of what it
+// rounds (the output's by its type), an eighth of what a bf16 product's would be.
+
 // Few query rows (single tokens, drafts): a tile of 16 rows; the waves of a
 // workgroup take the 32-key steps of its range in turn, each straight from the
 // cache into MFMA operands, with a running maximum and sum per row, and meet in
 // LDS once, at the end.  At 128 registers two workgroups fit a CU.
+// Bound by the cache's bytes and the latency of reading them: 32 sequences of 256
+// to 8192 keys, 8 KV heads of 128: 40 us for 137 MB (3.4 TB/s; workgroups with
+// equal work take 16 to 59 us, all started at once); one sequence of 16384 keys
+// in 32 splits 9.8 us (21 MB); 640 keys 7.5: about 3.7 us without any key, 1.2
+// per 256 keys.  Slower there: 16 waves, V's rows through LDS for wide loads (57
+// and 64 us in all where this was 53), all steps in 512 equal runs (45 against
+// 45 for the batch, but 17 against 13 for 16384 keys).
 constexpr int kRowWaves = 8;
 constexpr int kRowGroups = 1024;           // workgroups with keys that a batch's work is cut into
 
@@ -602,6 +627,11 @@ __global__ __launch_bounds__(64 * kRowWaves, SHORT ? 2 : 4) void kv4_attn_rows_k
 // NT r + n of the transposed block holds nibble n of word r: MFMA row r of
 // product n.  Two buffers, one barrier per block; the next block's codes are in
 // registers while this one is multiplied.
+// Bound by what is issued beside the MFMAs: 2011 tokens at 8192 keys, 32 heads on
+// 8 of 128, take 288 us, 820 TFLOP/s, where an 8192^3 fp16 product reaches 1170;
+// VALU (softmax and codes) is busy 68 % of the cycles, LDS 54 %, the MFMAs 38 %.  A
+// prompt of 512 takes 17 us: 8 blocks of keys at about 1.3 us each, and the
+// launch.  128 rows make a block's numbers once for twice as many products.
 constexpr int kBlock = 64;                 // keys
 
 template <int D, int CT, bool BF>
@@ -877,8 +907,11 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   }
 }
 
-// Joins the splits of a row: one workgroup per row, D / 4 lanes per split, so
-// that all partial results of the row are requested at once.
+// Joins the splits of a row: out = sum 2^(M_s - M) O_s / sum 2^(M_s - M) L_s.  One
+// workgroup per row, D / 4 lanes per split, so that all partial results of the
+// row are requested at once; in the order of the splits, so results repeat.  Bound
+// by its launch and two round trips: 3.3 us for 32 rows of 32 splits, 4.1 for
+// 1024 rows of 2.
 constexpr int kMaxSplits = 128;
 
 template <int D, bool BF>
@@ -961,11 +994,11 @@ bool rows_aligned(const void* p, int64_t sb, int64_t st, int64_t sh, int64_t siz
 //    1024 tokens of a prompt 30 (128 rows: 36), 1536 48 (50), 2048 76 (64).
 //  * Splits until two workgroups per CU are reached: 32 sequences of up to 8192
 //    keys in 2 splits 46, in 1 55, in 8 53; 64 of 2048 in 1 26, in 2 35, in 4 46.
-//  * A split has 256 keys or more for single tokens (4096 keys: 16 splits 9.3, 8
-//    10.6, 4 13), 512 in long caches (16384 keys: 32 splits 13, 64 13.7) and for
-//    wide tiles; and twice as many keys as there are rows, whose partial results
-//    are written and read once per split (256 tokens at 8192 keys: 4 splits 92, 1
-//    163; at 1024 keys: 2 splits 40, 1 25).
+//  * A split of a tile of 16 rows has 256 keys or more (4096 keys: 16 splits 9.3, 8
+//    10.6, 4 13), beyond 32 splits 512 (16384 keys: 32 splits 13, 64 13.7); one of
+//    a wide tile 512, and twice as many keys as there are rows, whose partial
+//    results are written and read once per split (256 tokens at 8192 keys: 4
+//    splits 92, 1 163; at 1024 keys: 2 splits 40, 1 25).
 //  * Up to 1024 keys the join of few rows costs what it saves (640 keys: 7.5
 //    without splits, 9.7 in 2, 8.3 in 8; 16 sequences of 1024: 11 and 13 in 2).
 struct Cut {
@@ -980,9 +1013,11 @@ Cut cut_of(int64_t batch, int64_t rows, int64_t tokens, int64_t KV, int64_t max_
                                                                      : 128;
   const int64_t keys = window > 0 ? std::min(max_len, window + tokens) : max_len;
   const int64_t tiles = (rows + tile - 1) / tile, wgs = std::max<int64_t>(batch * KV * tiles, 1);
-  const int64_t share = std::max<int64_t>(2 * rows, tile == 16 && keys <= 8192 ? 256 : 512);
-  int64_t want = std::min(512 / wgs, (keys + share - 1) / share);
-  if (tile == 16 && keys <= 1024) want = 1;
+  // (never fewer splits for more keys: the workspace is sized for a call without a window)
+  auto parts = [&](int64_t share) { return (keys + share - 1) / share; };
+  int64_t want = tile > 16 ? parts(std::max<int64_t>(512, 2 * rows))
+                 : keys <= 1024 ? 1 : std::max(std::min<int64_t>(parts(256), 32), parts(512));
+  want = std::min(512 / wgs, want);
   if (split > 0) want = split;
   want = std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
   return {(int)tile, (int)tiles, (int)want};
@@ -1077,7 +1112,7 @@ extern "C" int64_t bf16x_kv4_attention_workspace(int64_t batch, int64_t tokens, 
                                                  int64_t head_dim, int64_t max_len) {
   if (check_cache(batch, tokens, n_kv_heads, head_dim, max_len) || n_heads <= 0 || n_heads % n_kv_heads) return -1;
   const int64_t rows = tokens * (n_heads / n_kv_heads);
-  const Cut cut = cut_of(batch, rows, tokens, n_kv_heads, max_len, 0);       // (a window leaves fewer)
+  const Cut cut = cut_of(batch, rows, tokens, n_kv_heads, max_len, 0);       // (with a window there are no more)
   return cut.splits == 1 ? 0 : cut.splits * batch * n_kv_heads * rows * (head_dim + 2) * 4;
 }
 

@@ -19,6 +19,12 @@
 // by 1e-11 of the total at most, where an fp32 sum would move it by the
 // probability of an unlikely token.  The exponential is a Taylor polynomial of
 // degree 11 in fp64 (relative error 1e-14 on half an octave).
+//
+// 128 rows of 128256 fp32 logits with mixed settings: 88 us.  The first launch, 40
+// us (66 MB: 13 us at a copy's rate), is bound by the fp64 instructions of a
+// weight and its bin, about 60 per logit; the second, 45 us, by the chain of
+// small steps of a row whose list is long, one workgroup a row.  One row (bf16,
+// all three filters): 9 + 18 us, launches and round trips one after another.
 #include <cfloat>
 
 #include "bf16x_device.h"
@@ -31,6 +37,8 @@ using namespace bf16x;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
 
+// Bins of 1/32 neper: a threshold's bin holds some hundred tokens of a model's
+// row, and 1023 of them reach down to exp(-32).
 constexpr int kBins = 1024;               // of a chunk; the last one holds everything below the others
 constexpr int kRest = kBins - 1;
 constexpr int kGroup = 16;                // bins of a group, which all chunks cut at the same cells of the grid

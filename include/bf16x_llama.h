@@ -294,9 +294,10 @@ typedef struct {
  * kept weights passes u times their sum (u is cut to [0, 1)).  T = 0 (or
  * anything not above 0) takes the first maximum.  A logit of -inf or NaN is
  * never drawn; with a logit of +inf only the +inf tokens are.  A row without any
- * other logit gives token -1.  Weights are computed in fp64 and summed as
- * integers of 2^-44, so the result does not depend on an order of summation; a
- * token below 2^-45 of the likeliest is not drawn.
+ * other logit gives token -1.  Weights are computed in fp64, summed as integers
+ * of 2^-44 of the largest weight of a chunk of the row (a few thousand tokens),
+ * and over the chunks in fp64 in a fixed order, so that results repeat; a token
+ * below 2^-45 of its chunk's likeliest is not drawn.
  * token int64 [rows]; logprob fp32 [rows] or NULL: the logarithm of the token's
  * probability among the kept ones (0 for T = 0, -inf for token -1).
  * state (NULL: none; rows must be 1): int32[2] {position, number of tokens in

@@ -323,3 +323,15 @@ def test_long_cache_offsets():
     assert torch.equal(kk, kv4.read(small, _i32([0] * B), 40, dtype=FP)[0])
     vals = [x.permute(0, 2, 1, 3).double().cpu().numpy() for x in (kk, vv)]
     _check_attention(q.cpu(), cache, vals, [39] * B, got)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("window", [1000, 1025, 8100, 8191, 8200])
+def test_windows_in_a_long_cache(window, tokens):
+    """Windows a little shorter than the cache, at lengths where the split of the keys changes."""
+    L, D, KV, G = 8300, 64, 1, 4
+    k, v = (_rand(1, KV, L, D, seed=s, dtype=FP) for s in (51, 52))
+    cache, vals = _cache(k, v)
+    q = _rand(1, tokens, KV * G, D, seed=53)
+    got = kv4.attention(q.to(DEV), cache, _i32([L - tokens]), window=window)
+    _check_attention(q, cache, vals, [L - tokens], got, window=window)

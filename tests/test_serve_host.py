@@ -182,3 +182,14 @@ def test_entries_validate_before_launch():
     assert draw(n=L.bf16x_sample_workspace(1, 100) - 1) == _lib.ECAPACITY
     assert draw(rows=0, n_u=0) == _lib.OK
     assert L.bf16x_sample_workspace(1, 0) == -1 and L.bf16x_sample_workspace(70000, 100) == -1
+
+
+@pytest.mark.parametrize("batch,tokens,heads,kv", [(1, 1, 32, 8), (1, 5, 32, 8), (2, 16, 8, 2), (1, 17, 32, 8),
+                                                   (3, 100, 12, 4), (1, 700, 32, 8), (16, 1, 32, 8), (90, 1, 8, 8)])
+def test_workspace_never_shrinks(batch, tokens, heads, kv):
+    """A window makes a call see fewer keys, and its workspace is sized without it: fewer keys may need no more."""
+    f = _lib.lib().bf16x_kv4_attention_workspace
+    lengths = sorted({n + d for n in (1, 256, 512, 1024, 1536, 4096, 8192, 10000, 16384, 40000, 1 << 20)
+                      for d in (-1, 0, 1, 300) if n + d > 0})
+    sizes = [f(batch, tokens, heads, kv, 128, n) for n in lengths]
+    assert sizes == sorted(sizes)
