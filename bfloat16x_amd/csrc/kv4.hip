@@ -622,16 +622,18 @@ __global__ __launch_bounds__(64 * kRowWaves, SHORT ? 2 : 4) void kv4_attn_rows_k
 // Many query rows (prompts): a tile of 64 CT rows, 16 CT per wave as CT column
 // blocks of the MFMA; the cache goes through LDS in blocks of 64 keys, made
 // into fp16 once for all rows, K as rows (padded by 16 bytes) and V
-// transposed (rows of 128 bytes, 16-byte columns exchanged by the row's word, so
-// that neither the writes nor the operand reads of 8 lanes meet in a bank).  Row
-// NT r + n of the transposed block holds nibble n of word r: MFMA row r of
-// product n.  Two buffers, one barrier per block; the next block's codes are in
-// registers while this one is multiplied.
-// Bound by what is issued beside the MFMAs: 2011 tokens at 8192 keys, 32 heads on
-// 8 of 128, take 288 us, 820 TFLOP/s, where an 8192^3 fp16 product reaches 1170;
-// VALU (softmax and codes) is busy 68 % of the cycles, LDS 54 %, the MFMAs 38 %.  A
-// prompt of 512 takes 17 us: 8 blocks of keys at about 1.3 us each, and the
-// launch.  128 rows make a block's numbers once for twice as many products.
+// transposed (rows of 128 bytes, 16-byte columns exchanged by the row's word, the
+// rows of words 8 .. 15 one row on, so that the operand reads of 16 lanes meet in
+// no bank).  Row NT r + n of the transposed block holds nibble n of word r: MFMA
+// row r of product n.  Two buffers, one barrier per block; the next block's codes
+// are in registers while this one is multiplied.
+// Bound by VALU and MFMA instructions that take turns, at two waves a SIMD: 2011
+// tokens at 8192 keys, 32 heads on 8 of 128, take 288 to 295 us, 820 TFLOP/s, where
+// an 8192^3 fp16 product reaches 1170; VALU (softmax and codes) is busy 56 % of the
+// cycles, the MFMAs 37 %, LDS 45 and 17 more by conflicts (26 without that one row:
+// 64-row tiles 414 us instead of 395, 128-row ones the same).  A prompt of 512
+// takes 17 us: 8 blocks of keys at about 1.3 us each, and the launch.  128 rows make
+// a block's numbers once for twice as many products.
 constexpr int kBlock = 64;                 // keys
 
 template <int D, int CT, bool BF>
@@ -640,7 +642,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   constexpr int W = D / 32, NT = D / 16, KW = D / 32;           // KW: words of codes a thread stages of a key
   constexpr int KROW = 2 * D + 16, VROW = 2 * kBlock;
   __shared__ __attribute__((aligned(16))) uint8_t kls[2][kBlock * KROW];
-  __shared__ __attribute__((aligned(16))) uint8_t vls[2][D * VROW];
+  __shared__ __attribute__((aligned(16))) uint8_t vls[2][(D + 1) * VROW];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads fastest, so that a head's tiles share an XCD's L2 where there are 8; the last tiles, which see the most
@@ -669,7 +671,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   // another thread's where D is 64
   const Exponents ex;
   const int kkey = tid >> 2, kpart = tid & 3;
-  const int vw = tid & (D / 8 - 1), vhalf = D == 64 ? (tid >> 3) & 1 : 0, vr = vw + 8 * vhalf, vquad = tid >> 4;
+  const int vw = tid & (D / 8 - 1), vhalf = D == 64 ? (tid >> 3) & 1 : 0, vr = vw + 8 * vhalf;
+  const int vquad = (tid >> 4 & 1) << 2 | (tid >> 5 & 3) | tid >> 7 << 3;            // (lanes 16 .. 31 write the other 8 bytes)
   uint32_t kr[KW], ksr, vr_[4], vsr[4];
   // (rows past the cache's end are its last one: the blocks' bases are uniform, offsets inside a block 32 bits)
   auto load_k = [&](int blk) {
@@ -716,7 +719,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
   };
   auto store_v = [&](int slot) {
     const int col = 4 * (vquad >> 3) + (vquad & 3);
-    uint8_t* vd = vls[slot] + NT * vr * VROW + ((col ^ (vr & 7)) * 16) + ((vquad >> 2) & 1) * 8;
+    uint8_t* vd = vls[slot] + (NT * vr + (vr >> 3)) * VROW + ((col ^ (vr & 7)) * 16) + ((vquad >> 2) & 1) * 8;
     uint32_t two[2][NT];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -848,7 +851,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_tiles_kernel(AttnArgs a) {
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const h8 vv = *(const h8*)(vls[slot] + (NT * c + n) * VROW + (((4 * h + g) ^ (c & 7)) * 16));
+        const h8 vv = *(const h8*)(vls[slot] + (NT * c + (c >> 3) + n) * VROW + (((4 * h + g) ^ (c & 7)) * 16));
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct)
           o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[ct][h], o[ct][n], 0, 0, 0);
