@@ -190,12 +190,16 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
     float step = fmaxf(mx - lowf, 0.f) * (1.f / 15.f);
     asm("" : "+v"(step));                  // rounded to fp32, then to fp16: not in one v_fma_mixlo_f16
     const _Float16 sc = (_Float16)step;
-    const float scf = (float)sc;
+    // (x - minimum) / scale rounded as a division rounds it, with one reciprocal per group, refined once, and one
+    // correction per value: the same code for every scale's significand and every value within 4 steps of a half
+    const float scf = (float)sc, r0 = __builtin_amdgcn_rcpf(scf);
+    const float inv = scf > 0.f ? fmaf(fmaf(-scf, r0, 1.f), r0, r0) : 0.f;
     uint32_t w = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float n = scf > 0.f ? fminf(fmaxf(__builtin_rintf((x[e] - lowf) / scf), 0.f), 15.f) : 0.f;
-      w |= (uint32_t)n << (e & 1 ? 14 + 2 * e : 2 * e);
+      const float t = x[e] - lowf, n = t * inv;
+      const float code = fminf(fmaxf(__builtin_rintf(fmaf(fmaf(-scf, n, t), inv, n)), 0.f), 15.f);
+      w |= (uint32_t)code << (e & 1 ? 14 + 2 * e : 2 * e);
     }
     const int64_t out = (b * a.KV + hk) * a.max_len + p;
     (is_k ? a.kc : a.vc)[out * LR + l] = w;
