@@ -62,10 +62,12 @@ __device__ __forceinline__ h2 minimum_of(uint32_t w) { return as_h2(__builtin_am
 // ---------------------------------------------------------------------------
 // Append and read.  8 values per lane (one word of codes: 16 bytes of a 16-bit
 // type in one load), so D / 8 lanes per row; the 4 lanes of a group meet in two
-// quad exchanges.  Both are bound by memory, or by the launch and two dependent
-// round trips (the position, then the rows) where there are few tokens: with 32
-// + 16 heads of 128 bf16 values, 2048 tokens take 13.3 us to append (46 MB, 3.4
-// TB/s; a copy reaches 5.0) and 4.0 to read back (11 MB), one token 3.0 and 1.9.
+// quad exchanges.  Both are bound by VALU and memory together (the append was
+// VALU-bound, 13.4 us at 88 % busy, while it divided and rounded to bf16 in
+// integers), or by the launch and two dependent round trips (the position, then
+// the rows) where there are few tokens: with 32 + 16 heads of 128 bf16 values,
+// 2048 tokens take 11.4 to 12.6 us to append (46 MB, 3.8 TB/s; a copy reaches 5.0)
+// and 3.2 to 4.7 to read back (11 MB), one token 2.7 and 1.7.
 // Only the scale and the minimum are rounded below fp32 on the way in, to the
 // fp16 they are kept in, and the codes are taken against those rounded values,
 // so that their rounding costs no more than half a step of the code.
@@ -97,9 +99,10 @@ __device__ __forceinline__ void load8(const void* p, int64_t i, float (&x)[8]) {
   }
 }
 
+// (a NaN stays one, with bits of the conversion's own)
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (TYPE == BF16X_BF16) return f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16);
+  if constexpr (TYPE == BF16X_BF16) return pk_bf16(a, b);
   return as_u32(h2{(_Float16)a, (_Float16)b});
 }
 
@@ -136,7 +139,7 @@ struct AppendArgs {
 // A workgroup per token; its rows (heads of q, k and v) are taken 256 / LR at a
 // time, by gridDim.z workgroups where there are few tokens.  The table's row is
 // read once per lane for all of them, and no lane divides (a workgroup per 256 /
-// LR rows of any token: 15.8 us for the 2048 tokens, and 13.3 so).
+// LR rows of any token: 15.8 us for the 2048 tokens where this took 13.3).
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
 #pragma clang fp contract(off)             // the rotation's products are rounded one by one, as its definition says
@@ -144,6 +147,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
   const int l = threadIdx.x % LR, t = blockIdx.x, heads = a.H + 2 * a.KV;
   const int64_t b = blockIdx.y, bt = b * a.tokens + t, p = (int64_t)a.pos[b] + t;
   const bool upper = l >= LR / 2, inside = p >= 0 && p < a.max_len;
+  const int64_t q_row = b * a.q_sb + t * a.q_st, k_row = b * a.k_sb + t * a.k_st, v_row = b * a.v_sb + t * a.v_st;
   f4 cs[4];
   if (a.cos_sin) {
     const int64_t pc = p < 0 ? 0 : p >= a.cos_rows ? a.cos_rows - 1 : p;
@@ -156,8 +160,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
     const int hk = is_q ? h : is_k ? h - a.H : h - a.H - a.KV;
     if (!is_q && !inside) continue;        // (whole rows: the lanes of a group go together)
     const void* src = is_q ? a.q : is_k ? a.k : a.v;
-    const int64_t off = is_q ? b * a.q_sb + t * a.q_st + hk * a.q_sh
-                             : is_k ? b * a.k_sb + t * a.k_st + hk * a.k_sh : b * a.v_sb + t * a.v_st + hk * a.v_sh;
+    const int64_t off = (is_q ? q_row : is_k ? k_row : v_row) + hk * (is_q ? a.q_sh : is_k ? a.k_sh : a.v_sh);
     float x[8];
     load8<TYPE>(src, off + 8 * l, x);
     if (a.cos_sin && (is_q || is_k)) {
@@ -280,7 +283,7 @@ __device__ __forceinline__ void key_range(const AttnArgs& a, int b, int t, int& 
 
 template <bool BF>
 __device__ __forceinline__ uint32_t out2(float a, float b) {
-  return BF ? f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16) : as_u32(h2{(_Float16)a, (_Float16)b});
+  return pack2<BF ? BF16X_BF16 : BF16X_F16>(a, b);
 }
 
 // The query operand of a lane: 8 N values of its row brought to fp16 by the power
