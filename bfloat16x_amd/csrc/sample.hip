@@ -175,29 +175,36 @@ __device__ __forceinline__ double log_weight(float x, float m, double inv_t) {
   return x == m ? 0.0 : ((double)x - (double)m) * inv_t;
 }
 
-// exp(y) for -kSpan <= y <= 0.
-__device__ __forceinline__ double weight_of(double y) {
-  const double z = y * 1.4426950408889634074;
-  const double n = __builtin_rint(z);
-  const double r = (z - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return p * __longlong_as_double((long long)((int)n + 1023) << 52);
-}
-// A weight (0 .. 1) as an integer of 2^-44, rounded by the addition of 2^52.
-__device__ __forceinline__ u64 mass_of(double w) {
-  return (u64)__double_as_longlong(w * 0x1p44 + 0x1p52) & ((1ull << 52) - 1);
-}
+// exp(y) for -kSpan <= y <= 0.  The constants are scalars that the compiler cannot
+// see through: as literals, each would be moved to a vector register again for
+// every logit, a quarter of all instructions.
+struct Exponential {
+  double log2e = 1.4426950408889634074, ln2 = 0.69314718055994530942, whole = 0x1p52, c[9] = {
+      1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0, 1.0 / 120.0,
+      1.0 / 24.0, 1.0 / 6.0};
+  __device__ __forceinline__ Exponential() {
+    asm("" : "+s"(log2e), "+s"(ln2), "+s"(whole));
+#pragma unroll
+    for (int i = 0; i < 9; ++i) asm("" : "+s"(c[i]));
+  }
+  __device__ __forceinline__ double times(double y, int power) const {          // exp(y) 2^power
+    const double z = y * log2e;
+    const double n = __builtin_rint(z);
+    const double r = (z - n) * ln2;
+    double p = c[0];
+#pragma unroll
+    for (int i = 1; i < 9; ++i) p = fma(p, r, c[i]);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)n + power);
+  }
+  __device__ __forceinline__ double operator()(double y) const { return times(y, 0); }
+  // exp(y) as an integer of 2^-44, rounded by the addition of 2^52; 0 for a y out of range (or NaN)
+  __device__ __forceinline__ u64 mass(double y) const {
+    return y >= -kSpan ? (u64)__double_as_longlong(times(y, 44) + whole) & ((1ull << 52) - 1) : 0;
+  }
+};
 
 template <class T>
 __device__ __forceinline__ T shfl_xor_t(T v, int o) {
@@ -306,6 +313,7 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
   }
   if (s.greedy) return;
   const double top = cell_of(mx, s.bins);
+  const Exponential weight_of;
   u64 sum = 0, rest = 0;
   uint32_t rest_count = 0;
 #pragma unroll
@@ -314,10 +322,11 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
     for (int e = 0; e < 8; ++e) {
       if (!(x[v][e] > -INFINITY)) continue;
       const double y = log_weight(x[v][e], mx, s.inv_t);
-      const u64 m = y >= -kSpan ? mass_of(weight_of(y)) : 0;
+      const u64 m = weight_of.mass(y);
       sum += m;
       if (!bins_on) continue;
-      const int b = bin_of(x[v][e], top, s.bins);
+      // (bin_of for a logit of at most mx)
+      const int b = x[v][e] == mx ? 0 : (int)fmin(top - cell_of(x[v][e], s.bins), (double)kRest);
       if (b == kRest) {                   // (often most of the row: not one address for all)
         rest += m;
         ++rest_count;
@@ -362,6 +371,7 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
 // bit by bit, a pass over the row each, first for top-k, then for top-p.
 template <int TYPE>
 __device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, float mx, const void* p, bool vec, u64* red) {
+  const Exponential weight_of;
   auto above = [&](u64 thr, u64& mass) {
     u64 n = 0, m = 0, total;
     for (int i = 8 * (int)threadIdx.x; i < a.vocab; i += 8 * kDrawT) {
@@ -372,7 +382,7 @@ __device__ u64 threshold_by_passes(const SampleArgs& a, const Setting& s, float 
         if (x[e] > -INFINITY && place_of(x[e], i + e) >= thr) {
           const double y = log_weight(x[e], mx, s.inv_t);
           ++n;
-          m += y >= -kSpan ? mass_of(weight_of(y)) : 0;
+          m += weight_of.mass(y);
         }
     }
     block_prefix<kDrawT>(m, red, mass);
@@ -470,11 +480,9 @@ __global__ __launch_bounds__(kDrawT) void sample_draw_kernel(SampleArgs a) {
   }
   double total;
   block_prefix<kDrawT>(share, redd, total);
+  const Exponential weight_of;
   // mass of a token in units of its chunk's maximum, and its weight
-  auto own_mass = [&](float x, float m_c) {
-    const double y = log_weight(x, m_c, s.inv_t);
-    return y >= -kSpan ? mass_of(weight_of(y)) : 0;
-  };
+  auto own_mass = [&](float x, float m_c) { return weight_of.mass(log_weight(x, m_c, s.inv_t)); };
   auto passes_min = [&](float x) {
     if (!s.m_on) return true;
     const double y = log_weight(x, mx, s.inv_t);
