@@ -20,11 +20,12 @@
 // probability of an unlikely token.  The exponential is a Taylor polynomial of
 // degree 11 in fp64 (relative error 1e-14 on half an octave).
 //
-// 128 rows of 128256 fp32 logits with mixed settings: 88 us.  The first launch, 40
-// us (66 MB: 13 us at a copy's rate), is bound by the fp64 instructions of a
-// weight and its bin, about 60 per logit; the second, 45 us, by the chain of
-// small steps of a row whose list is long, one workgroup a row.  One row (bf16,
-// all three filters): 9 + 18 us, launches and round trips one after another.
+// 128 rows of 128256 fp32 logits with mixed settings: 82 us.  The first launch, 36
+// us (66 MB: 13 us at a copy's rate), is bound by the instructions of a weight and
+// its bin, about 45 per logit, most of them fp64, and the LDS atomics; the second,
+// 46 us, by the chain of small steps of a row whose list is long, one workgroup a
+// row.  One row (bf16, all three filters): 8 + 18 us, launches and round trips one
+// after another.
 #include <cfloat>
 
 #include "bf16x_device.h"
@@ -47,7 +48,7 @@ constexpr int kOpen = kBins / kGroup - 1; // groups of a row; the tokens below t
 constexpr int kList = 4096;               // tokens of the thresholds' bins that are sorted in LDS
 // A list of kRanked tokens is sorted by counting alone; a longer one by kCells
 // cells of its range if none has more than kFull tokens (128 rows of mixed
-// settings 88 us; bitonically, which very uneven lists are left to, 96).
+// settings took 88 us so, and 96 bitonically, which uneven lists are left to).
 constexpr int kRanked = 512;
 constexpr int kCells = 2048;
 constexpr int kFull = 64;
@@ -200,9 +201,9 @@ struct Exponential {
     return __builtin_ldexp(p, (int)n + power);
   }
   __device__ __forceinline__ double operator()(double y) const { return times(y, 0); }
-  // exp(y) as an integer of 2^-44, rounded by the addition of 2^52; 0 for a y out of range (or NaN)
+  // exp(y) as an integer of 2^-44, rounded by the addition of 2^52: 0 for a y under -31, or NaN
   __device__ __forceinline__ u64 mass(double y) const {
-    return y >= -kSpan ? (u64)__double_as_longlong(times(y, 44) + whole) & ((1ull << 52) - 1) : 0;
+    return (u64)__double_as_longlong(times(fmax(y, -kSpan), 44) + whole) & ((1ull << 52) - 1);
   }
 };
 
@@ -313,28 +314,34 @@ __global__ __launch_bounds__(kT) void sample_chunk_kernel(SampleArgs a) {
   }
   if (s.greedy) return;
   const double top = cell_of(mx, s.bins);
+  const float under = mx > -INFINITY ? mx : 0.f;                // (a chunk without a token has no weight)
   const Exponential weight_of;
   u64 sum = 0, rest = 0;
   uint32_t rest_count = 0;
+  // (eight weights at a time, without branches between them)
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+  for (int v = 0; v < NV; ++v) {
+    u64 m[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (!(x[v][e] > -INFINITY)) continue;
-      const double y = log_weight(x[v][e], mx, s.inv_t);
-      const u64 m = weight_of.mass(y);
-      sum += m;
-      if (!bins_on) continue;
-      // (bin_of for a logit of at most mx)
+      m[e] = weight_of.mass(log_weight(x[v][e], under, s.inv_t));
+      sum += m[e];
+    }
+    if (!bins_on) continue;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // (bin_of for a logit of at most mx; not for what is no token)
       const int b = x[v][e] == mx ? 0 : (int)fmin(top - cell_of(x[v][e], s.bins), (double)kRest);
+      if (!(x[v][e] > -INFINITY)) continue;
       if (b == kRest) {                   // (often most of the row: not one address for all)
-        rest += m;
+        rest += m[e];
         ++rest_count;
       } else {
-        atomicAdd(&hm[b], m);
+        atomicAdd(&hm[b], m[e]);
         if (s.k_on) atomicAdd(&hc[b], 1u);
       }
     }
+  }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     sum += shfl_xor_t(sum, o);
